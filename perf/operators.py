@@ -175,7 +175,7 @@ def _prepare_attn(c, g):
         from molten_b200 import kv
         s["ctx"] = _context()
         s["cache"] = kv.KvCache(kc, vc, s["ks"], s["vs"])
-        s["ws"] = kv.paged_attention_workspace(H, K, D, DEV)
+        s["ws"] = kv.paged_attention_workspace(D, DEV)
     return s
 
 
