@@ -120,6 +120,8 @@ def _prepare_plan(c, g):
     s = dict(lens=lens, new=new, table=table.contiguous(), free=free, n_free=n_free, blocks=blocks, seq=_i32(R), n_free_out=_i32(1),
              row_start=_i32(R + 1), positions=_i32(total), token_req=_i32(total), kv_lens=_i32(total),
              slots=torch.zeros(total, dtype=torch.int64, device=DEV), done=None, lens_mid=_i32(R), n_free_mid=_i32(1))
+    # the program's table: a pass finds it as the last one left it, the plan writes the same entries again
+    s["table_out"] = s["table"].clone()
     if c["release"]:
         s["done"] = (torch.rand(R, generator=g, device=DEV) < 0.1).int()
     return s
@@ -365,9 +367,9 @@ def _own_plan(s):
     if s["done"] is not None:
         kv.kv_release(s["ctx"], s["done"], lens, bs, s["table"], s["free"], n_free, s["lens_mid"], s["n_free_mid"])
         lens, n_free = s["lens_mid"], s["n_free_mid"]
-    kv.kv_plan(s["ctx"], lens, s["new"], bs, s["table"], s["free"], n_free, s["seq"], s["n_free_out"], s["row_start"], s["positions"],
+    kv.kv_plan(s["ctx"], lens, s["new"], bs, s["table_out"], s["free"], n_free, s["seq"], s["n_free_out"], s["row_start"], s["positions"],
                s["token_req"], s["kv_lens"], s["slots"])
-    return dict(seq=s["seq"], n_free=s["n_free_out"], table=s["table"], free=s["free"], row_start=s["row_start"], positions=s["positions"],
+    return dict(seq=s["seq"], n_free=s["n_free_out"], table=s["table_out"], free=s["free"], row_start=s["row_start"], positions=s["positions"],
                 token_req=s["token_req"], kv_lens=s["kv_lens"], slots=s["slots"])
 
 
