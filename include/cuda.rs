@@ -23,6 +23,15 @@ pub const MC_ROUTE_SOFTMAX_RENORM: c_int = 0;
 pub const MC_ROUTE_SIGMOID_BIAS: c_int = 1;
 pub const MC_DTYPE_BF16: c_int = 0;
 pub const MC_DTYPE_F32: c_int = 1;
+pub const MC_DTYPE_E4M3: c_int = 2;
+pub const MC_KV_NO_PAGES: c_int = 1;
+pub const MC_KV_TABLE_FULL: c_int = 2;
+pub const MC_KV_ROWS_FULL: c_int = 4;
+pub const MC_KV_BAD_LENGTH: c_int = 8;
+pub const MC_KV_LIST_FULL: c_int = 16;
+pub const MC_KV_BAD_SLOT: c_int = 32;
+pub const MC_KV_BAD_PAGE: c_int = 64;
+pub const MC_KV_BAD_ROW: c_int = 128;
 pub const MC_TEST_SKIP_LOGIT_PUBLISH: c_int = 1;
 pub const MC_TEST_SKIP_BARRIER_ARRIVE: c_int = 2;
 
@@ -508,6 +517,49 @@ extern "C" {
     pub fn mc_set_wait_limit(ctx: *mut McCtx, ns: u64) -> c_int;
     pub fn mc_set_test_flags(ctx: *mut McCtx, flags: c_int) -> c_int;
     pub fn mc_eval_math(ctx: *mut McCtx, op: c_int, x: *const f32, y: *mut f32, n: c_int) -> c_int;
+    pub fn mc_kv_plan(
+        ctx: *mut McCtx, lens: *const i32, new_lens: *const i32, n_req: c_int, block_size: c_int,
+        block_table: *mut i32, table_width: c_int, free_list: *const i32, n_free: *const i32,
+        free_len: c_int, seq_lens: *mut i32, n_free_out: *mut i32, row_start: *mut i32,
+        positions: *mut i32, token_req: *mut i32, kv_lens: *mut i32, slots: *mut u64,
+        max_tokens: c_int, status: *mut u32,
+    ) -> c_int;
+    pub fn mc_kv_release(
+        ctx: *mut McCtx, done: *const u32, lens: *const i32, n_req: c_int, block_size: c_int,
+        block_table: *const i32, table_width: c_int, free_list: *mut i32, n_free: *const i32,
+        free_len: c_int, lens_out: *mut i32, n_free_out: *mut i32, status: *mut u32,
+    ) -> c_int;
+    pub fn mc_rope_turns(theta: f32, position_scale: f32, rot_dim: c_int, out: *mut u64) -> c_int;
+    pub fn mc_qk_norm_rope(
+        ctx: *mut McCtx, q: *const u16, q_stride: usize, k: *const u16, k_stride: usize,
+        v: *const u16, v_stride: usize, n_tokens: c_int, n_heads: c_int, n_kv_heads: c_int,
+        head_dim: c_int, q_norm_w: *const u16, k_norm_w: *const u16, eps: f32,
+        positions: *const i32, turns: *const u64, rot_dim: c_int, interleaved: c_int,
+        q_out: *mut u16, q_out_stride: usize, slots: *const u64, k_cache: *mut c_void,
+        v_cache: *mut c_void, kv_dtype: c_int, num_blocks: c_int, block_size: c_int,
+        block_stride: usize, k_scale: *const f32, v_scale: *const f32, status: *mut u32,
+    ) -> c_int;
+    pub fn mc_paged_attention_workspace_bytes(head_dim: c_int) -> usize;
+    pub fn mc_paged_attention(
+        ctx: *mut McCtx, q: *const u16, q_stride: usize, n_rows: c_int, n_heads: c_int,
+        k_cache: *const c_void, v_cache: *const c_void, kv_dtype: c_int, num_blocks: c_int,
+        block_size: c_int, block_stride: usize, n_kv_heads: c_int, head_dim: c_int,
+        k_scale: *const f32, v_scale: *const f32, block_table: *const i32, n_req: c_int,
+        table_width: c_int, kv_lens: *const i32, row_req: *const i32, window: c_int, scale: f32,
+        out: *mut u16, out_stride: usize, lse: *mut f32, workspace: *mut c_void, ws_bytes: usize,
+        status: *mut u32,
+    ) -> c_int;
+    pub fn mc_logits_process(
+        ctx: *mut McCtx, logits: *const c_void, logits_stride: usize, dtype: c_int, vocab: c_int,
+        batch: c_int, seen: *const u32, counts: *const u16, repetition: *const f32,
+        frequency: *const f32, presence: *const f32, bias_start: *const i32, bias_ids: *const u32,
+        bias_vals: *const f32, n_bias: c_int, allowed: *const u32, allowed_row: *const i32,
+        n_allowed: c_int, out: *mut c_void, out_stride: usize, keys: *mut u64,
+    ) -> c_int;
+    pub fn mc_logits_mark(
+        ctx: *mut McCtx, tokens: *const u32, batch: c_int, seen: *mut u32, counts: *mut u16,
+        vocab: c_int,
+    ) -> c_int;
 }
 
 /// The library's error for a nonzero return code, with its message.

@@ -50,6 +50,18 @@ extern "C" {
 
 #define MC_DTYPE_BF16 0
 #define MC_DTYPE_F32 1
+#define MC_DTYPE_E4M3 2 /* 8-bit float (paged cache) */
+
+/* Status bits of the paged-cache calls (a nullable device word the kernels OR
+ * into; the caller clears it). */
+#define MC_KV_NO_PAGES 1    /* kv_plan: the free list ran out; requests refused */
+#define MC_KV_TABLE_FULL 2  /* kv_plan: a request is longer than the block table is wide */
+#define MC_KV_ROWS_FULL 4   /* kv_plan: more token rows than max_tokens */
+#define MC_KV_BAD_LENGTH 8  /* a negative length, or one beyond the block table */
+#define MC_KV_LIST_FULL 16  /* kv_release: more pages than the free list holds */
+#define MC_KV_BAD_SLOT 32   /* qk_norm_rope: a slot outside the cache (row not written) */
+#define MC_KV_BAD_PAGE 64   /* paged_attention: a page outside the cache (its keys left out) */
+#define MC_KV_BAD_ROW 128   /* paged_attention: row_req outside the block table (row empty) */
 
 typedef struct mc_ctx mc_ctx;
 
@@ -299,6 +311,135 @@ int mc_sample_draw(mc_ctx* ctx, const uint16_t* logits, int vocab, const uint32_
  * device position by one. */
 int mc_sample_mark(mc_ctx* ctx, const uint32_t* tok, uint32_t* seen, int vocab,
                    uint32_t* pos_dev);
+
+/* --------------------------------- paged key-value cache and attention
+ * What a batched decode step needs between the Q/K/V projections and the
+ * output projection. No counterpart one to one in the reference, whose
+ * decode attention (sdpa_vector_norm_rope) norms, rotates and attends over
+ * one contiguous cache in one dispatch.
+ *
+ * The cache: k_cache and v_cache hold pages [num_blocks][n_kv_heads]
+ * [block_size][head_dim], page p at p * block_stride elements (block_stride
+ * >= n_kv_heads * block_size * head_dim and a multiple of 16 bytes, so K and
+ * V pages may alternate in one allocation). block_size is any positive
+ * number; head_dim 64 or 128; kv_dtype MC_DTYPE_BF16, or MC_DTYPE_E4M3 with
+ * optional scales f32[n_kv_heads] (stored = value / scale, saturating; read =
+ * stored * scale). With num_blocks = 1 and block_size = max_seq it is the
+ * cache mc_proj3_gemv_scatter writes. Slot s is row s % block_size of page
+ * s / block_size; all ones means "not written". A request's block table row
+ * lists its pages in order. */
+
+/* One step's bookkeeping, on the device. For request r holding lens[r]
+ * tokens and adding new_lens[r] (NULL: one each) takes the pages it needs
+ * from the free list -- a stack of page numbers, free_list[0 .. *n_free) free,
+ * with room for free_len -- from the top and in request order, writes them into
+ * block_table[r][..] (row width table_width) and sets seq_lens[r] = lens[r] +
+ * new_lens[r], *n_free_out, row_start[n_req + 1] (the first token row of each
+ * request; rows are packed in request order) and for each token row
+ * t < max_tokens: positions[t], token_req[t] (its request), kv_lens[t] =
+ * positions[t] + 1 and slots[t]. Rows behind the last one get position 0,
+ * token_req -1, kv_len 0 and no slot, so launches of a fixed size may run
+ * over them.
+ * A request is admitted whole or not at all. One that the free list, the
+ * table or max_tokens cannot take keeps its length and pages; its rows stay
+ * in place with kv_len 0 and no slot, and a status bit says why. Pages are
+ * counted over the requests in order, refused ones included, so one that is
+ * refused for pages also refuses every later one that needs any. seq_lens
+ * may be lens and n_free_out may be n_free (a captured step then advances by
+ * itself); with other buffers a call may be repeated. */
+int mc_kv_plan(mc_ctx* ctx, const int32_t* lens, const int32_t* new_lens, int n_req,
+               int block_size, int32_t* block_table, int table_width, const int32_t* free_list,
+               const int32_t* n_free, int free_len, int32_t* seq_lens, int32_t* n_free_out,
+               int32_t* row_start, int32_t* positions, int32_t* token_req, int32_t* kv_lens,
+               uint64_t* slots, int max_tokens, uint32_t* status);
+/* Gives the pages of the requests with done[r] != 0 back to the free list
+ * (pushed in request order, each request's first page first) and sets their
+ * lens_out to 0; the other lengths are copied. lens_out may be lens and
+ * n_free_out may be n_free. */
+int mc_kv_release(mc_ctx* ctx, const uint32_t* done, const int32_t* lens, int n_req,
+                  int block_size, const int32_t* block_table, int table_width,
+                  int32_t* free_list, const int32_t* n_free, int free_len, int32_t* lens_out,
+                  int32_t* n_free_out, uint32_t* status);
+
+/* Host helper: the frequencies position_scale * theta^(-2 i / rot_dim), i <
+ * rot_dim / 2, as fractions of a turn per position in 64-bit fixed point
+ * (2^64 is one turn), the `turns` table of mc_qk_norm_rope (upload it once;
+ * any other frequencies may be given the same way). */
+int mc_rope_turns(float theta, float position_scale, int rot_dim, uint64_t* out);
+/* Per-head RMSNorm of Q and K with gains [head_dim] (a NULL gain: no norm),
+ * rotation of their first rot_dim dimensions (a multiple of 16, 0: none) by
+ * positions[t], pairs (i, i + rot_dim / 2) or with `interleaved` (2i, 2i + 1),
+ * and the cache write, for n_tokens rows: q [n_tokens][n_heads][head_dim] ->
+ * q_out; k -> k_cache and v -> v_cache (as they are; v NULL: not written) at
+ * slots[t] (NULL: slot t). Computed in fp32, rounded once where stored. The
+ * *_stride are elements between tokens (multiples of 8), so q, k and v may be
+ * parts of one fused projection row. q_out is q itself, with its stride, or
+ * apart from q, k and v. Angles are exact modulo a turn at any position.
+ * Every row of q_out is written, also those without a slot. Slots are
+ * distinct; of two tokens with one slot either may stay, or parts of both. */
+int mc_qk_norm_rope(mc_ctx* ctx, const uint16_t* q, size_t q_stride, const uint16_t* k,
+                    size_t k_stride, const uint16_t* v, size_t v_stride, int n_tokens,
+                    int n_heads, int n_kv_heads, int head_dim, const uint16_t* q_norm_w,
+                    const uint16_t* k_norm_w, float eps, const int32_t* positions,
+                    const uint64_t* turns, int rot_dim, int interleaved, uint16_t* q_out,
+                    size_t q_out_stride, const uint64_t* slots, void* k_cache, void* v_cache,
+                    int kv_dtype, int num_blocks, int block_size, size_t block_stride,
+                    const float* k_scale, const float* v_scale, uint32_t* status);
+
+/* Softmax attention of n_rows query rows [n_heads][head_dim] over the cache:
+ * row r reads the first kv_lens[r] keys of block table row row_req[r] (NULL:
+ * r), the last `window` of them if window > 0; query head h uses KV head
+ * h / (n_heads / n_kv_heads). out[r] (bf16) and optional lse[r][n_heads]
+ * (natural log of the summed exponentials of scale * q.k). A row without keys
+ * (or with row_req -1) gives zeros and lse -inf. Several rows of one request
+ * (draft tokens, a short prompt) read their keys each for itself. Keys of
+ * pages outside [0, num_blocks) are left out; nothing behind kv_lens is read.
+ * A non-finite K or V element of a key that is read makes the results it
+ * enters non-finite. out must not overlap q. workspace: zeroed once,
+ * mc_paged_attention_workspace_bytes(head_dim) device bytes, 16-byte aligned,
+ * owned by one chain of ordered calls (each call leaves its counters zero
+ * again; captured graphs that may run at once need one each). */
+size_t mc_paged_attention_workspace_bytes(int head_dim);
+int mc_paged_attention(mc_ctx* ctx, const uint16_t* q, size_t q_stride, int n_rows, int n_heads,
+                       const void* k_cache, const void* v_cache, int kv_dtype, int num_blocks,
+                       int block_size, size_t block_stride, int n_kv_heads, int head_dim,
+                       const float* k_scale, const float* v_scale, const int32_t* block_table,
+                       int n_req, int table_width, const int32_t* kv_lens,
+                       const int32_t* row_req, int window, float scale, uint16_t* out,
+                       size_t out_stride, float* lse, void* workspace, size_t ws_bytes,
+                       uint32_t* status);
+
+/* ------------------------------------------------- rules on logits
+ * The requests' penalties, biases and grammar masks on a batch of logits
+ * rows [batch][vocab] (dtype MC_DTYPE_BF16 or MC_DTYPE_F32, row strides in
+ * elements) before argmax or mc_sample_draw. For token i of row b, in fp32:
+ *   seen bit i (u32 bitmap [batch][ceil(vocab/32)]): v > 0 ? v / repetition[b]
+ *     : v * repetition[b];
+ *   counts[b][i] > 0 (u16): v - frequency[b] * count - presence[b];
+ *   + the biases bias_vals[j] of the entries j in bias_start[b] ..
+ *     bias_start[b + 1] (of n_bias) with bias_ids[j] = i; ids ascend within a
+ *     row, equal ids add up in order (which entries of an unsorted row count
+ *     is not specified); ids beyond the vocabulary are left out;
+ *   -inf where bit i of mask row allowed_row[b] (NULL: b) of `allowed` (u32
+ *     bitmap [n_allowed][ceil(vocab/32)], 1: allowed) is 0; a row outside
+ *     [0, n_allowed) has no mask.
+ * Stored in the logits' type to out (logits itself, or apart from it). NULL
+ * leaves a rule out; seen and repetition go together, counts with a frequency
+ * or a presence penalty. keys (nullable): keys[b], zero on entry, takes the
+ * greedy key of the stored row as mc_gemv_head_argmax leaves it (ties to the
+ * lowest id, NaN never; a row that the mask leaves nothing gives token 0). */
+int mc_logits_process(mc_ctx* ctx, const void* logits, size_t logits_stride, int dtype,
+                      int vocab, int batch, const uint32_t* seen, const uint16_t* counts,
+                      const float* repetition, const float* frequency, const float* presence,
+                      const int32_t* bias_start, const uint32_t* bias_ids,
+                      const float* bias_vals, int n_bias, const uint32_t* allowed,
+                      const int32_t* allowed_row, int n_allowed, void* out, size_t out_stride,
+                      unsigned long long* keys);
+/* Counts the drawn tokens[batch]: sets their bits in seen and adds one to
+ * their counts (saturating at 65535); either may be NULL. Tokens outside the
+ * vocabulary are left out. */
+int mc_logits_mark(mc_ctx* ctx, const uint32_t* tokens, int batch, uint32_t* seen,
+                   uint16_t* counts, int vocab);
 
 /* ----------------------------------------------------------- prefill path */
 

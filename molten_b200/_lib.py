@@ -25,6 +25,16 @@ ROUTE_SOFTMAX_RENORM = 0
 ROUTE_SIGMOID_BIAS = 1
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
+DTYPE_E4M3 = 2
+
+KV_NO_PAGES = 1
+KV_TABLE_FULL = 2
+KV_ROWS_FULL = 4
+KV_BAD_LENGTH = 8
+KV_LIST_FULL = 16
+KV_BAD_SLOT = 32
+KV_BAD_PAGE = 64
+KV_BAD_ROW = 128
 
 
 class McError(RuntimeError):
@@ -131,6 +141,17 @@ SIGNATURES: dict[str, tuple] = {
     "mc_set_wait_limit": (I, [P, C.c_ulonglong]),
     "mc_set_test_flags": (I, [P, I]),
     "mc_copy_async": (I, [P, P, P, C.c_size_t]),
+    "mc_kv_plan": (I, [P, P, P, I, I, P, I, P, P, I, P, P, P, P, P, P, P, I, P]),
+    "mc_kv_release": (I, [P, P, P, I, I, P, I, P, P, I, P, P, P]),
+    "mc_rope_turns": (I, [F, F, I, P]),
+    "mc_qk_norm_rope": (I, [P, P, C.c_size_t, P, C.c_size_t, P, C.c_size_t, I, I, I, I, P, P, F,
+                            P, P, I, I, P, C.c_size_t, P, P, P, I, I, I, C.c_size_t, P, P, P]),
+    "mc_paged_attention_workspace_bytes": (C.c_size_t, [I]),
+    "mc_paged_attention": (I, [P, P, C.c_size_t, I, I, P, P, I, I, I, C.c_size_t, I, I, P, P, P,
+                               I, I, P, P, I, F, P, C.c_size_t, P, P, C.c_size_t, P]),
+    "mc_logits_process": (I, [P, P, C.c_size_t, I, I, I, P, P, P, P, P, P, P, P, I, P, P, I, P,
+                              C.c_size_t, P]),
+    "mc_logits_mark": (I, [P, P, I, P, P, I]),
     "mc_gemm_q4_workspace_words": (C.c_size_t, [I]),
     "mc_gemm_q4": (I, [P, P, I, QP, P, P, C.c_size_t, P]),
 }

@@ -18,6 +18,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
+from .kv import _on, _ptr
 from .lfm import Context, _p, ensure
 
 MIN_TEMPERATURE = 1e-6
@@ -119,3 +120,80 @@ class SampleScratch:
         set, and advances the device position ``pos`` (int32 [1]) when given."""
         ensure(tok.numel() == 1 and tok.dtype == torch.int32, "sampled token slot")
         _lib.call("mc_sample_mark", self.ctx.handle, _p(tok), _p(self.seen), self.vocab, _p(pos))
+
+
+@dataclass
+class LogitsRules:
+    """The rules of a batch of requests on their logits rows [batch, vocab];
+    None leaves a rule out.
+
+    ``seen``: u32 bitmap (int32 [batch, ceil(vocab / 32)]) of the tokens that
+    ``repetition`` (f32 [batch]) divides (positive logits) or multiplies;
+    ``counts``: u16 counts (int16 [batch, vocab]) for ``frequency`` and
+    ``presence`` (f32 [batch]); ``bias_start`` (int32 [batch + 1]),
+    ``bias_ids`` (int32, ascending within a row) and ``bias_values`` (f32): the
+    biases of row b are the entries bias_start[b] .. bias_start[b + 1];
+    ``allowed``: u32 bitmap (int32 [masks, ceil(vocab / 32)]), 0 bits become
+    -inf; ``allowed_row`` (int32 [batch]): the mask of each row (-1: none;
+    None: mask b for row b)."""
+    seen: torch.Tensor | None = None
+    counts: torch.Tensor | None = None
+    repetition: torch.Tensor | None = None
+    frequency: torch.Tensor | None = None
+    presence: torch.Tensor | None = None
+    bias_start: torch.Tensor | None = None
+    bias_ids: torch.Tensor | None = None
+    bias_values: torch.Tensor | None = None
+    allowed: torch.Tensor | None = None
+    allowed_row: torch.Tensor | None = None
+
+
+def _rows2(ctx: Context, t: torch.Tensor, what: str) -> tuple[int, int]:
+    ensure(t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1),
+           f"{what}: rows [batch, vocab], each contiguous")
+    ensure(_on(ctx, t), f"{what} must be on {ctx.device}")
+    return t.data_ptr(), t.stride(0)
+
+
+def logits_process(ctx: Context, logits: torch.Tensor, out: torch.Tensor, rules: LogitsRules,
+                   best: torch.Tensor | None = None) -> None:
+    """Applies ``rules`` to ``logits`` [batch, vocab] (bf16 or f32) into
+    ``out`` (logits itself, or apart from it): repetition, frequency and
+    presence, biases, then the grammar mask. ``best`` (int64 [batch], zero on
+    entry): takes the greedy keys that lfm.token_tail reads."""
+    B, V = logits.shape
+    ensure(logits.dtype in (torch.bfloat16, torch.float32) and out.dtype == logits.dtype and
+           out.shape == logits.shape, "logits_process: logits and out, BF16 or F32")
+    lp, ls = _rows2(ctx, logits, "logits")
+    op, os = _rows2(ctx, out, "out")
+    W = (V + 31) // 32
+    i32, f32 = torch.int32, torch.float32
+    r = rules
+    n_bias = 0 if r.bias_ids is None else r.bias_ids.numel()
+    ensure(r.allowed is None or (r.allowed.dim() == 2 and r.allowed.shape[1] == W),
+           "allowed shape")
+    _lib.call("mc_logits_process", ctx.handle, lp, ls,
+              _lib.DTYPE_BF16 if logits.dtype == torch.bfloat16 else _lib.DTYPE_F32, V, B,
+              _ptr(ctx, r.seen, i32, "seen", B * W),
+              _ptr(ctx, r.counts, torch.int16, "counts", B * V),
+              _ptr(ctx, r.repetition, f32, "repetition", B),
+              _ptr(ctx, r.frequency, f32, "frequency", B),
+              _ptr(ctx, r.presence, f32, "presence", B),
+              _ptr(ctx, r.bias_start, i32, "bias_start", B + 1),
+              _ptr(ctx, r.bias_ids, i32, "bias_ids"),
+              _ptr(ctx, r.bias_values, f32, "bias_values", n_bias), n_bias,
+              _ptr(ctx, r.allowed, i32, "allowed"),
+              _ptr(ctx, r.allowed_row, i32, "allowed_row", B),
+              0 if r.allowed is None else r.allowed.shape[0], op, os,
+              _ptr(ctx, best, torch.int64, "best", B))
+
+
+def logits_mark(ctx: Context, tokens: torch.Tensor, rules: LogitsRules, vocab: int) -> None:
+    """Adds the drawn ``tokens`` (int32 [batch]) to the rules' seen bitmap and
+    counts (a no-op for rules that go by neither)."""
+    if rules.seen is None and rules.counts is None:
+        return
+    B = tokens.numel()
+    _lib.call("mc_logits_mark", ctx.handle, _ptr(ctx, tokens, torch.int32, "tokens"), B,
+              _ptr(ctx, rules.seen, torch.int32, "seen", B * ((vocab + 31) // 32)),
+              _ptr(ctx, rules.counts, torch.int16, "counts", B * vocab), vocab)
