@@ -32,6 +32,7 @@ pub const MC_KV_LIST_FULL: c_int = 16;
 pub const MC_KV_BAD_SLOT: c_int = 32;
 pub const MC_KV_BAD_PAGE: c_int = 64;
 pub const MC_KV_BAD_ROW: c_int = 128;
+pub const MC_KV_WAIT: c_int = 256;
 pub const MC_TEST_SKIP_LOGIT_PUBLISH: c_int = 1;
 pub const MC_TEST_SKIP_BARRIER_ARRIVE: c_int = 2;
 

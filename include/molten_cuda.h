@@ -62,6 +62,7 @@ extern "C" {
 #define MC_KV_BAD_SLOT 32   /* qk_norm_rope: a slot outside the cache (row not written) */
 #define MC_KV_BAD_PAGE 64   /* paged_attention: a page outside the cache (its keys left out) */
 #define MC_KV_BAD_ROW 128   /* paged_attention: row_req outside the block table (row empty) */
+#define MC_KV_WAIT 256      /* paged_attention: a copy did not arrive in time (results NaN) */
 
 typedef struct mc_ctx mc_ctx;
 

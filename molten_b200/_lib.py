@@ -35,6 +35,7 @@ KV_LIST_FULL = 16
 KV_BAD_SLOT = 32
 KV_BAD_PAGE = 64
 KV_BAD_ROW = 128
+KV_WAIT = 256
 
 
 class McError(RuntimeError):

@@ -43,26 +43,40 @@ PS_HD long long ps_begin(long long U, int c, int G) { return U / G * c + U % G *
 // The CTA whose range holds unit u (0 <= u < U, G <= U).
 PS_HD int ps_owner(long long u, long long U, int G) { return (int)(((u + 1) * G - 1) / U); }
 
-// One CTA's piece of an item.
-struct PsPiece {
-  int row, item;           // query row, item within the row
-  int unit, units;         // first unit of the piece within the item, unit count
-  int first_cta, last_cta; // CTAs that hold the item (equal: the item is whole)
+// Walks the pieces of one CTA: the item, its units in this CTA, and how many
+// units of the range are left from the piece's first one on.
+struct PsCursor {
+  int row, item;    // query row, item within the row
+  int n;            // units of each of the row's items
+  int unit, units;  // first unit of the piece within the item, unit count
+  long long left;
 };
 
-// The piece that starts at unit u of a row whose units start at row_start
-// (n units for each item) and ends by u_end.
-PS_HD PsPiece ps_piece(long long u, long long u_end, int row, long long row_start, int n,
-                       long long U, int G) {
-  PsPiece p;
-  const long long in_row = u - row_start;
-  p.row = row;
-  p.item = (int)(in_row / n);
-  p.unit = (int)(in_row % n);
-  const long long left = u_end - u;
-  p.units = left < n - p.unit ? (int)left : n - p.unit;
-  const long long a = row_start + (long long)p.item * n;
-  p.first_cta = ps_owner(a, U, G);
-  p.last_cta = ps_owner(a + n - 1, U, G);
-  return p;
+// The piece that starts `in_row` units after the start of row `row` (n units
+// an item), with `left` units of the range to go.
+PS_HD PsCursor ps_first(int row, long long in_row, int n, long long left) {
+  PsCursor c;
+  c.row = row;
+  c.n = n;
+  c.item = (int)(in_row / n);
+  c.unit = (int)(in_row - (long long)c.item * n);
+  c.left = left;
+  c.units = left < n - c.unit ? (int)left : n - c.unit;
+  return c;
+}
+
+// Steps to the next piece; false at the range's end. A row is done after
+// `items` items; units_of(row) gives the next row's n.
+template <typename F>
+PS_HD bool ps_next(PsCursor& c, int items, F&& units_of) {
+  c.left -= c.units;
+  if (c.left <= 0) return false;
+  c.unit = 0;
+  if (++c.item == items) {
+    c.item = 0;
+    ++c.row;
+    c.n = units_of(c.row);
+  }
+  c.units = c.left < c.n ? (int)c.left : c.n;
+  return true;
 }

@@ -26,7 +26,8 @@ STATUS_BITS = {
     _lib.KV_NO_PAGES: "the free list ran out", _lib.KV_TABLE_FULL: "a request outgrew its block table",
     _lib.KV_ROWS_FULL: "more token rows than the maps hold", _lib.KV_BAD_LENGTH: "a bad length",
     _lib.KV_LIST_FULL: "more pages than the free list holds", _lib.KV_BAD_SLOT: "a slot outside the cache",
-    _lib.KV_BAD_PAGE: "a page outside the cache", _lib.KV_BAD_ROW: "a row of no request"}
+    _lib.KV_BAD_PAGE: "a page outside the cache", _lib.KV_BAD_ROW: "a row of no request",
+    _lib.KV_WAIT: "a copy did not arrive in time"}
 
 
 def raise_on_status(status: torch.Tensor, what: str) -> None:

@@ -27,56 +27,53 @@ static void run(const std::vector<int>& lens, long long capacity, int window, in
   long long U = 0;
   for (int r = 0; r < R; ++r) U += (long long)ps_units(ps_row(lens[r], capacity, window), unit) * items;
   const int G = (int)std::min<long long>(grid, U);
-  std::map<std::pair<int, int>, std::vector<std::pair<int, PsPiece>>> of;  // item -> (cta, piece)
+  auto units_of = [&](int r) {
+    CHECK(r < R);
+    return ps_units(ps_row(lens[r], capacity, window), unit);
+  };
+  std::map<std::pair<int, int>, std::vector<std::pair<int, PsCursor>>> of;  // item -> (cta, piece)
   long long covered = 0;
   for (int c = 0; c < G; ++c) {
-    long long u = ps_begin(U, c, G);
-    const long long u_end = ps_begin(U, c + 1, G);
-    CHECK(u < u_end);
-    CHECK(ps_owner(u, U, G) == c && ps_owner(u_end - 1, U, G) == c);
+    const long long u0 = ps_begin(U, c, G), u_end = ps_begin(U, c + 1, G);
+    CHECK(u0 < u_end);
+    CHECK(ps_owner(u0, U, G) == c && ps_owner(u_end - 1, U, G) == c);
     int row = 0;
     long long start = 0;
     for (;;) {
-      const long long n = (long long)ps_units(ps_row(lens[row], capacity, window), unit) * items;
-      if (u < start + n) break;
+      const long long n = (long long)units_of(row) * items;
+      if (u0 < start + n) break;
       start += n;
       ++row;
     }
     int continued = 0, joined_in = 0;
-    while (u < u_end) {
-      const PsRow keys = ps_row(lens[row], capacity, window);
-      const int n = ps_units(keys, unit);
-      if (u >= start + (long long)n * items) {
-        start += (long long)n * items;
-        ++row;
-        CHECK(row < R);
-        continue;
-      }
-      const PsPiece p = ps_piece(u, u_end, row, start, n, U, G);
-      CHECK(p.units >= 1 && p.unit >= 0 && p.unit + p.units <= n && p.item < items);
-      CHECK(p.first_cta <= c && c <= p.last_cta);
-      CHECK((p.unit == 0) == (c == p.first_cta));
-      CHECK((p.unit + p.units == n) == (c == p.last_cta));
-      if (p.first_cta != p.last_cta) (c == p.first_cta ? continued : joined_in)++;
-      of[{row, p.item}].push_back({c, p});
+    PsCursor p = ps_first(row, u0 - start, units_of(row), u_end - u0);
+    do {
+      CHECK(p.units >= 1 && p.unit >= 0 && p.unit + p.units <= p.n && p.item < items);
+      CHECK(p.n == units_of(p.row) && p.left == u_end - u0 - (covered - u0));
+      const bool begins = p.unit == 0, ends = p.unit + p.units == p.n;
+      // what the kernel asks of an item that is not whole in this CTA
+      const long long u = u_end - p.left;
+      CHECK((ps_owner(u - p.unit, U, G) == c) == begins);
+      CHECK((ps_owner(u - p.unit + p.n - 1, U, G) == c) == ends);
+      if (!(begins && ends)) (begins ? continued : joined_in)++;
+      of[{p.row, p.item}].push_back({c, p});
       covered += p.units;
-      u += p.units;
-    }
+    } while (ps_next(p, items, units_of));
+    CHECK(covered == u_end);
     CHECK(continued <= 1 && joined_in <= 1);
   }
   CHECK(covered == U);
   CHECK((long long)of.size() == (long long)R * items);
   std::set<int> counters;
   for (auto& [key, pieces] : of) {
-    int at = 0, cta = pieces[0].second.first_cta;
+    int at = 0, cta = pieces[0].first;
     for (auto& [c, p] : pieces) {
       CHECK(p.unit == at && c == cta);
       at += p.units;
       ++cta;
     }
-    CHECK(at == ps_units(ps_row(lens[key.first], capacity, window), unit));
-    CHECK(cta - 1 == pieces[0].second.last_cta);
-    if (pieces.size() > 1) CHECK(counters.insert(pieces[0].second.first_cta).second);
+    CHECK(at == units_of(key.first));
+    if (pieces.size() > 1) CHECK(counters.insert(pieces[0].first).second);
   }
 }
 
