@@ -178,6 +178,13 @@ __device__ __forceinline__ int v_dim(int nt, int n) {
   return 64 * (nt / 8) + 8 * n + nt % 8;
 }
 
+// Folds (m2, l2) into a running maximum and sum.
+__device__ __forceinline__ void fold(float& m, float& l, float m2, float l2) {
+  const float top = fmaxf(m, m2), use = top == -INFINITY ? 0.0f : top;
+  l = __fmaf_rn(l, ex2(m - use), ex2(m2 - use) * l2);
+  m = top;
+}
+
 template <int D, bool F8>
 __global__ void __launch_bounds__(Shape<D, F8>::kThreads, kPerSm)
 paged_attention_kernel(const PaParams P) {
@@ -245,7 +252,7 @@ paged_attention_kernel(const PaParams P) {
   if (u0 >= incl - mine && u0 < incl) {
     long long at = incl - mine;
     int r = r_lo;
-    for (;; ++r) {
+    for (; r < r_hi - 1; ++r) {
       const long long n = (long long)units_of(r) * P.items;
       if (u0 < at + n) break;
       at += n;
@@ -258,7 +265,7 @@ paged_attention_kernel(const PaParams P) {
   // ---- filling the ring: the step at fill_base of the piece `fill`
   uint8_t* ring = ring_s + (size_t)warp * S::kStages * S::kStage;
   const uint64_t policy = mc_policy_evict_normal();
-  PsCursor fill = ps_first(row_s, in_row_s, units_of(row_s), u_end - u0);
+  PsCursor fill = ps_first(row_s, in_row_s, units_of(row_s), P.items, u_end - u0);
   PsCursor piece = fill;
   int fill_base = 0, fill_hi = 0, fill_head = 0, page = -1;
   uint32_t filled = 0;
@@ -275,7 +282,7 @@ paged_attention_kernel(const PaParams P) {
   // to the next step of this warp; its page numbers are on their way afterwards
   auto seek = [&]() {
     while (more && fill_base >= fill_hi) {
-      more = ps_next(fill, P.items, units_of);
+      more = ps_next(fill, P.items, P.rows, units_of);
       if (more) enter();
     }
     const int tok = fill_base + lane;
@@ -568,22 +575,63 @@ paged_attention_kernel(const PaParams P) {
     __syncthreads();
     if (!last_s) continue;
     __threadfence();
-    for (int i = tid; i < kHeads * D; i += S::kThreads) {
-      const int h = i / D, d = i % D;
-      float mx = -INFINITY, sum = 0.0f, val = 0.0f;
-      for (int x = first_cta; x <= last_cta; ++x) {
-        const float* pp = P.parts + part_floats(D) * (2 * (size_t)x + (x == first_cta ? 1 : 0));
-        const float mc = __ldcg(pp + kHeads * D + h);
-        const float m2 = fmaxf(mx, mc);
-        const float use = m2 == -INFINITY ? 0.0f : m2;
-        const float a = ex2(mx - use), b = ex2(mc - use);
-        sum = __fmaf_rn(sum, a, b * __ldcg(pp + kHeads * D + kHeads + h));
-        val = __fmaf_rn(val, a, b * __ldcg(pp + i));
-        mx = m2;
+    auto part_of = [&](int x) {
+      return P.parts + part_floats(D) * (2 * (size_t)x + (x == first_cta ? 1 : 0));
+    };
+    {  // the largest m and the sum, head tid % 8, pieces tid / 8, tid / 8 + threads / 8, ...
+      const int h = tid % kHeads;
+      float mx = -INFINITY, sum = 0.0f;
+      for (int x = first_cta + tid / kHeads; x <= last_cta; x += S::kThreads / kHeads) {
+        const float* pp = part_of(x) + kHeads * D + h;
+        fold(mx, sum, __ldcg(pp), __ldcg(pp + kHeads));
       }
-      finish(h, d, mx, sum, val);
+#pragma unroll
+      for (int d = kHeads; d < 32; d <<= 1)
+        fold(mx, sum, __shfl_xor_sync(0xffffffffu, mx, d), __shfl_xor_sync(0xffffffffu, sum, d));
+      if (lane < kHeads) {
+        m_s[warp][lane] = mx;
+        l_s[warp][lane] = sum;
+      }
     }
-  } while (ps_next(piece, P.items, units_of));
+    __syncthreads();
+    // four elements a thread, 8 pieces' loads in flight
+    for (int i = tid; i < heads * D / 4; i += S::kThreads) {
+      const int h = 4 * i / D;
+      float mx = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < S::kWarps; ++w)
+        fold(mx, sum, m_s[w][h], l_s[w][h]);
+      const float use = mx == -INFINITY ? 0.0f : mx;
+      float4 val = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int x0 = first_cta; x0 <= last_cta; x0 += 8) {
+        float4 v[8];
+        float m8[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int x = x0 + k;
+          m8[k] = -INFINITY;
+          v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (x <= last_cta) {
+            v[k] = __ldcg(reinterpret_cast<const float4*>(part_of(x)) + i);
+            m8[k] = __ldcg(part_of(x) + kHeads * D + h);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float a = ex2(m8[k] - use);
+          val.x = __fmaf_rn(a, v[k].x, val.x);
+          val.y = __fmaf_rn(a, v[k].y, val.y);
+          val.z = __fmaf_rn(a, v[k].z, val.z);
+          val.w = __fmaf_rn(a, v[k].w, val.w);
+        }
+      }
+      const int d = 4 * i % D;
+      finish(h, d, mx, sum, val.x);
+      finish(h, d + 1, mx, sum, val.y);
+      finish(h, d + 2, mx, sum, val.z);
+      finish(h, d + 3, mx, sum, val.w);
+    }
+  } while (ps_next(piece, P.items, P.rows, units_of));
   if (gave_up) {  // copies still on their way end before the shared memory goes
     for (uint32_t i = filled > S::kStages ? filled - S::kStages : 0; i < filled; ++i)
       wait_full(&full_s[warp][i % S::kStages], (i / S::kStages) & 1, P.wait_ns);

@@ -41,7 +41,10 @@ PS_HD int ps_units(PsRow r, int unit) {
 PS_HD long long ps_begin(long long U, int c, int G) { return U / G * c + U % G * c / G; }
 
 // The CTA whose range holds unit u (0 <= u < U, G <= U).
-PS_HD int ps_owner(long long u, long long U, int G) { return (int)(((u + 1) * G - 1) / U); }
+PS_HD int ps_owner(long long u, long long U, int G) {
+  const long long c = ((u + 1) * G - 1) / U;
+  return c < 0 ? 0 : c < G ? (int)c : G - 1;
+}
 
 // Walks the pieces of one CTA: the item, its units in this CTA, and how many
 // units of the range are left from the piece's first one on.
@@ -54,27 +57,30 @@ struct PsCursor {
 
 // The piece that starts `in_row` units after the start of row `row` (n units
 // an item), with `left` units of the range to go.
-PS_HD PsCursor ps_first(int row, long long in_row, int n, long long left) {
+PS_HD PsCursor ps_first(int row, long long in_row, int n, int items, long long left) {
   PsCursor c;
   c.row = row;
   c.n = n;
-  c.item = (int)(in_row / n);
-  c.unit = (int)(in_row - (long long)c.item * n);
+  const long long item = in_row / n;
+  c.item = item < items ? (int)item : items - 1;
+  c.unit = item < items ? (int)(in_row - item * n) : n - 1;
   c.left = left;
   c.units = left < n - c.unit ? (int)left : n - c.unit;
   return c;
 }
 
-// Steps to the next piece; false at the range's end. A row is done after
-// `items` items; units_of(row) gives the next row's n.
+// Steps to the next piece; false at the range's end, and after the last of
+// `rows` rows whatever the units say (lengths that another stream changes
+// meanwhile give wrong results, but no index out of range). A row is done
+// after `items` items; units_of(row) gives the next row's n.
 template <typename F>
-PS_HD bool ps_next(PsCursor& c, int items, F&& units_of) {
+PS_HD bool ps_next(PsCursor& c, int items, int rows, F&& units_of) {
   c.left -= c.units;
   if (c.left <= 0) return false;
   c.unit = 0;
   if (++c.item == items) {
     c.item = 0;
-    ++c.row;
+    if (++c.row >= rows) return false;
     c.n = units_of(c.row);
   }
   c.units = c.left < c.n ? (int)c.left : c.n;

@@ -46,7 +46,7 @@ static void run(const std::vector<int>& lens, long long capacity, int window, in
       ++row;
     }
     int continued = 0, joined_in = 0;
-    PsCursor p = ps_first(row, u0 - start, units_of(row), u_end - u0);
+    PsCursor p = ps_first(row, u0 - start, units_of(row), items, u_end - u0);
     do {
       CHECK(p.units >= 1 && p.unit >= 0 && p.unit + p.units <= p.n && p.item < items);
       CHECK(p.n == units_of(p.row) && p.left == u_end - u0 - (covered - u0));
@@ -58,7 +58,7 @@ static void run(const std::vector<int>& lens, long long capacity, int window, in
       if (!(begins && ends)) (begins ? continued : joined_in)++;
       of[{p.row, p.item}].push_back({c, p});
       covered += p.units;
-    } while (ps_next(p, items, units_of));
+    } while (ps_next(p, items, R, units_of));
     CHECK(covered == u_end);
     CHECK(continued <= 1 && joined_in <= 1);
   }
