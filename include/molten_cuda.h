@@ -321,7 +321,7 @@ int mc_sample_mark(mc_ctx* ctx, const uint32_t* tok, uint32_t* seen, int vocab,
  *
  * The cache: k_cache and v_cache hold pages [num_blocks][n_kv_heads]
  * [block_size][head_dim], page p at p * block_stride elements (block_stride
- * >= n_kv_heads * block_size * head_dim and a multiple of 16 bytes, so K and
+ * >= n_kv_heads * block_size * head_dim and a multiple of head_dim, so K and
  * V pages may alternate in one allocation). block_size is any positive
  * number; head_dim 64 or 128; kv_dtype MC_DTYPE_BF16, or MC_DTYPE_E4M3 with
  * optional scales f32[n_kv_heads] (stored = value / scale, saturating; read =

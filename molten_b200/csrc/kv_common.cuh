@@ -56,13 +56,14 @@ static inline int mc_check_kv_cache(const char* name, const void* k, const void*
   MC_REQUIRE(k && v, "%s: null cache", name);
   MC_REQUIRE(mc_aligned(k, 16) && mc_aligned(v, 16), "%s: the cache must be 16-byte aligned", name);
   const size_t page = (size_t)n_kv_heads * (size_t)block_size * (size_t)head_dim;
-  const size_t lane = dtype == MC_DTYPE_BF16 ? 8 : 16;  // elements of 16 bytes
   MC_REQUIRE(block_stride >= page || num_blocks == 1,
              "%s: block stride %zu below a page of %zu elements", name, block_stride, page);
-  MC_REQUIRE(block_stride % lane == 0, "%s: block stride %zu not a multiple of 16 bytes", name,
-             block_stride);
-  MC_REQUIRE(block_stride <= ((size_t)1 << 62) / (size_t)num_blocks,
-             "%s: block stride %zu out of range", name, block_stride);
+  MC_REQUIRE(block_stride % (size_t)head_dim == 0,
+             "%s: block stride %zu not a multiple of head_dim", name, block_stride);
+  // rows are numbered in 32 bits (the memory of a GPU holds fewer of 64 bytes)
+  MC_REQUIRE(page / head_dim < 0xffffffffull &&
+                 block_stride / head_dim * (num_blocks - 1) + page / head_dim < 0xffffffffull,
+             "%s: a cache of more than 2^32 - 2 rows", name);
   MC_REQUIRE(dtype == MC_DTYPE_E4M3 || (!k_scale && !v_scale),
              "%s: scales belong to an e4m3 cache", name);
   MC_REQUIRE(mc_aligned(k_scale, 4) && mc_aligned(v_scale, 4), "%s: scales misaligned", name);

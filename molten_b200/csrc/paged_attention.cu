@@ -20,13 +20,12 @@
 // by byte permutes.
 //
 // Memory. Every warp has a ring of steps in shared memory that its own lanes
-// fill with 1-D bulk copies, one for each run of keys that lie together in a
-// page (8 keys at most): deep enough that an SM has 60 KB and more in flight,
-// and filled across the borders of pieces, so that the next item's keys
-// arrive while the last one is joined. The 8-key parts of a step start 32
-// bytes (mod 128) apart, and a lane takes its keys from the part lane % 4:
-// the 4 rows x 2 chunks that a quarter-warp reads from V fall into different
-// banks although whole rows are multiples of 128 bytes.
+// fill with 16-byte asynchronous copies, deep enough that an SM has 60 KB and
+// more on their way, and filled across the borders of pieces, so that the next
+// item's keys arrive while the last one is joined. (1-D bulk copies, one for
+// each run of keys that lie together in a page, took as long for pages of 16
+// keys and up, 14% longer for e4m3 rows of 64 bytes, and 1.7 times as long for
+// pages of one key: a copy costs an SM some 47 cycles whatever its size.)
 //
 // Rounding of P. Eight heads fill rows 0-7 of the 16-row tile; P is split
 // into high and low parts (bf16 + bf16, or f16 + f16 for an e4m3 cache) and
@@ -51,7 +50,7 @@
 
 namespace {
 
-constexpr int kMaxCtas = 512;
+constexpr int kMaxCtas = 1024;
 constexpr int kHeads = 8;               // query heads of an item
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -67,7 +66,8 @@ struct PaParams {
   const void* kc;
   const void* vc;
   int num_blocks, block_size;
-  size_t block_stride;
+  uint32_t page_rows;  // block_stride / D
+  PsDiv by_block;
   const float* k_scale;
   const float* v_scale;
   const int32_t* table;
@@ -143,27 +143,36 @@ __device__ __forceinline__ void e4m3x4_to_f16(uint32_t v, uint32_t& lo, uint32_t
       : "r"(v));
 }
 
-constexpr int kPart = 8;              // keys of a part
-constexpr int kStep = 4 * kPart;      // keys a warp takes at once, one a lane
-constexpr int kPerSm = 2;             // CTAs an SM holds at once
-
-// Shape of the kernel for a head dimension and cache type: warps and ring
-// depth fill the shared memory of two CTAs an SM.
+// Shape of the kernel for a head dimension and cache type: 8 warps an SM with
+// rings that hold 128 to 192 KB, except e4m3 rows of 64 bytes, whose time goes
+// into instructions more than into bytes and which take 12 warps (97 -> 85 us
+// for 64 rows of 6100 keys x 8 heads; bf16 rows at 12 warps and shallower rings
+// 51 -> 54 us for 131071 keys). Rows of 256 bytes take 16 keys a step, so that
+// 4 warps' rings fit twice (94 -> 87 us for 131071 keys).
+//
+// A step's K, and its V, are 128-byte lines of 8 chunks (16 bytes; chunk ch of
+// key k is number k kChunks + ch). A line's chunks are permuted, number n at
+// n ^ turn with turn = 2 (k / kPart), ^ 4 for an odd key if a row is whole
+// lines, so that the 8 chunks a quarter-warp reads at once (2 keys x 4 chunks
+// of K, 4 parts x 2 chunks of V) fall into different banks.
 template <int D, bool F8>
 struct Shape {
-  static constexpr int kRow = D * (F8 ? 1 : 2);          // bytes of a key's row
-  static constexpr int kPartBytes = kPart * kRow + 32;
-  static constexpr int kHalf = 4 * kPartBytes;           // K or V of a step
+  static constexpr int kRow = D * (F8 ? 1 : 2);   // bytes of a key's row
+  static constexpr int kChunks = kRow / 16;       // 16-byte chunks of a row
+  static constexpr int kStep = kRow == 256 ? 16 : 32;  // keys a warp takes at once, one a lane
+  static constexpr int kPart = kStep / 4;         // keys a lane's V fragments come from
+  static constexpr int kHalf = kStep * kRow;      // K or V of a step
   static constexpr int kStage = 2 * kHalf;
-  static constexpr int kWarps = D == 128 && !F8 ? 3 : 4;
-  static constexpr int kStages = D == 64 ? (F8 ? 5 : 3) : 2;
+  static constexpr int kWarps = 4;
+  static constexpr int kStages = kRow == 64 ? 4 : D == 64 ? 3 : 2;
+  static constexpr int kPerSm = kRow == 64 ? 3 : 2;  // CTAs an SM holds at once
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kUnit = kWarps * kStep;           // keys of a unit
-  static constexpr int kORow = D + 4;                    // floats of a row in o
+  static constexpr int kUnit = kWarps * kStep;    // keys of a unit
+  static constexpr int kORow = D + 4;             // floats of a row in o
   static constexpr size_t kRingBytes = (size_t)kWarps * kStages * kStage;
   static constexpr size_t kOBytes = (size_t)kWarps * kHeads * kORow * sizeof(float);
   static constexpr size_t kSmem = kRingBytes + kOBytes;
-  static_assert(kPerSm * (kSmem + 2048) <= 228 * 1024, "two CTAs an SM");
+  static_assert(kPerSm * (kSmem + 2048) <= 228 * 1024, "shared memory");
 };
 
 __device__ __forceinline__ uint32_t word(const uint4& u, int i) {
@@ -186,10 +195,12 @@ __device__ __forceinline__ void fold(float& m, float& l, float m2, float l2) {
 }
 
 template <int D, bool F8>
-__global__ void __launch_bounds__(Shape<D, F8>::kThreads, kPerSm)
+__global__ void __launch_bounds__(Shape<D, F8>::kThreads, (Shape<D, F8>::kPerSm))
 paged_attention_kernel(const PaParams P) {
   using S = Shape<D, F8>;
   constexpr int kT = D / 8;              // n-tiles of P.V
+  constexpr int kZ = S::kStep / 16;
+  constexpr uint32_t kAll = (1u << S::kPart) - 1;
   constexpr int kKLoads = S::kRow / 64;  // 16-byte loads of a lane's K row part
   constexpr int kVWords = S::kRow / 32;  // words of a lane's V row part
   extern __shared__ __align__(128) uint8_t ring_s[];
@@ -202,7 +213,7 @@ paged_attention_kernel(const PaParams P) {
   __shared__ int row_s;
   __shared__ uint32_t last_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid < S::kWarps * S::kStages) mc_mbar_init(&full_s[0][0] + tid, 1);
+  if (tid < S::kWarps * S::kStages) mc_mbar_init(&full_s[0][0] + tid, 32);
   mc_fence_barrier_init();
   mc_pdl_launch_dependents();
   mc_pdl_wait();
@@ -264,19 +275,18 @@ paged_attention_kernel(const PaParams P) {
 
   // ---- filling the ring: the step at fill_base of the piece `fill`
   uint8_t* ring = ring_s + (size_t)warp * S::kStages * S::kStage;
-  const uint64_t policy = mc_policy_evict_normal();
   PsCursor fill = ps_first(row_s, in_row_s, units_of(row_s), P.items, u_end - u0);
   PsCursor piece = fill;
-  int fill_base = 0, fill_hi = 0, fill_head = 0, page = -1;
-  uint32_t filled = 0;
+  int fill_base = 0, fill_hi = 0, fill_stage = 0, page = -1;
+  uint32_t filled = 0, in_page = 0, head_row = 0;
   bool more = true;
   const int32_t* table = nullptr;
   auto enter = [&]() {  // the piece `fill`
     const PsRow keys = row_of(fill.row);
     const int lo = keys.low + fill.unit * S::kUnit;
     fill_hi = (int)min((long long)keys.len, (long long)lo + (long long)fill.units * S::kUnit);
-    fill_base = lo + warp * kStep;
-    fill_head = fill.item / P.subs;
+    fill_base = lo + warp * S::kStep;
+    head_row = (uint32_t)(fill.item / P.subs) * P.block_size;
     table = P.table + (size_t)(P.row_req ? max(P.row_req[fill.row], 0) : fill.row) * P.width;
   };
   // to the next step of this warp; its page numbers are on their way afterwards
@@ -286,33 +296,41 @@ paged_attention_kernel(const PaParams P) {
       if (more) enter();
     }
     const int tok = fill_base + lane;
-    page = more && tok < fill_hi ? table[tok / P.block_size] : -1;
+    page = -1;
+    if (more && lane < S::kStep && tok < fill_hi) {
+      const int b = ps_div(tok, P.by_block);
+      in_page = (uint32_t)(tok - b * P.block_size);
+      page = table[b];
+    }
   };
+  // this lane copies chunk number lane + 32 i of the step, key i kKeys + lane / kChunks
+  constexpr int kKeys = 32 / S::kChunks;
+  const uint8_t* kc = static_cast<const uint8_t*>(P.kc) + 16 * (lane % S::kChunks);
+  const uint8_t* vc = static_cast<const uint8_t*>(P.vc) + 16 * (lane % S::kChunks);
   auto issue = [&]() {
-    const int stage = filled % S::kStages;
-    const int tok = fill_base + lane, in_page = tok % P.block_size;
-    const bool live = tok < fill_hi && page >= 0 && page < P.num_blocks;
-    if (tok < fill_hi && !live && P.status) atomicOr(P.status, MC_KV_BAD_PAGE);
+    const int tok = fill_base + lane;
+    const bool there = lane < S::kStep && tok < fill_hi;
+    const bool live = there && page >= 0 && page < P.num_blocks;
+    if (there && !live && P.status) atomicOr(P.status, MC_KV_BAD_PAGE);
     const uint32_t all = __ballot_sync(0xffffffffu, live);
-    uint64_t* bar = &full_s[warp][stage];
-    if (lane == 0) {
-      live_s[warp][stage] = all;
-      mc_mbar_expect_tx(bar, 2 * S::kRow * __popc(all));
+    if (lane == 0) live_s[warp][fill_stage] = all;
+    const uint32_t row = live ? (uint32_t)page * P.page_rows + head_row + in_page : 0xffffffffu;
+    uint8_t* to = ring + fill_stage * S::kStage;
+    const int odd = S::kChunks >= 8 ? 4 * ((lane / S::kChunks) & 1) : 0;
+#pragma unroll
+    for (int i = 0; i < S::kStep / kKeys; ++i) {
+      const int key = i * kKeys + lane / S::kChunks;
+      const uint32_t r = __shfl_sync(0xffffffffu, row, key);
+      const int turn = 2 * (key / S::kPart) ^ odd;
+      const int at = 512 * i + 16 * (lane ^ turn);
+      if (r != 0xffffffffu) {
+        mc_cp_async16(to + at, kc + (size_t)r * S::kRow);
+        mc_cp_async16(to + S::kHalf + at, vc + (size_t)r * S::kRow);
+      }
     }
-    // a run starts a part, a page, or follows a key that is left out
-    const bool starts =
-        live && (lane % kPart == 0 || in_page == 0 || !((all >> (lane - 1)) & 1u));
-    const uint32_t stops = __ballot_sync(0xffffffffu, starts || !live) >> lane >> 1;
-    __syncwarp();
-    if (starts) {
-      const int n = min(stops ? __ffs(stops) : kPart, kPart - lane % kPart);
-      const size_t off = ((size_t)page * P.block_stride +
-                          ((size_t)fill_head * P.block_size + in_page) * D) * (F8 ? 1 : 2);
-      uint8_t* to = ring + stage * S::kStage + lane / kPart * S::kPartBytes + lane % kPart * S::kRow;
-      mc_bulk_g2s(to, static_cast<const uint8_t*>(P.kc) + off, n * S::kRow, bar, policy);
-      mc_bulk_g2s(to + S::kHalf, static_cast<const uint8_t*>(P.vc) + off, n * S::kRow, bar, policy);
-    }
+    mc_cp_async_arrive(&full_s[warp][fill_stage]);
     ++filled;
+    fill_stage = fill_stage + 1 == S::kStages ? 0 : fill_stage + 1;
     fill_base += S::kUnit;
     seek();
   };
@@ -320,9 +338,27 @@ paged_attention_kernel(const PaParams P) {
   seek();
   for (int i = 0; i < S::kStages && more; ++i) issue();
 
-  uint32_t used = 0;
+  int stage = 0;
+  uint32_t phase = 0;
   bool gave_up = false;
   const int c = lane & 3, hr = lane >> 2;
+  // Where this lane reads: K key kPart (hr / 2) + hr % 2 (+ 4 z + 2 j), chunk c (+ 4 i: the other
+  // half of the line for odd i); V key kPart c (+ 4 z + i), chunk hr (+ 8 n), or half a chunk.
+  constexpr bool kHalfChunk = F8 && D == 64;
+  const int k_turn = 16 * (c ^ (2 * (hr >> 1)) ^ (S::kChunks >= 8 ? 4 * (hr & 1) : 0));
+  const int k_at = S::kChunks >= 8 ? (S::kPart * (hr >> 1) + (hr & 1)) * S::kRow + k_turn
+                                   : (S::kPart * (hr >> 1)) * S::kRow + (k_turn ^ (64 * (hr & 1)));
+  const int k_flip = (k_at ^ 64) - k_at;
+  const int v_at = S::kPart * c * S::kRow +
+                   (kHalfChunk ? 16 * ((hr >> 1) ^ (2 * c)) + 8 * (hr & 1) : 16 * (hr ^ (2 * c)));
+  const int v_flip = (v_at ^ 64) - v_at;
+  auto finish = [&](int row, int head, int kvh, int d, float mx, float sum, float val) {
+    const float vscale = F8 && P.v_scale ? P.v_scale[kvh] : 1.0f;
+    const float r = sum == 0.0f ? 0.0f : __fdiv_rn(val, sum) * vscale;
+    P.out[(size_t)row * P.out_stride + (size_t)head * D + d] = mc_f32_to_bf16(r);
+    if (P.lse && d == 0)
+      P.lse[(size_t)row * P.H + head] = sum == 0.0f ? -INFINITY : __fmaf_rn(mx, kLn2, logf(sum));
+  };
   do {
     const PsRow keys = row_of(piece.row);
     const int row = piece.row;
@@ -379,6 +415,15 @@ paged_attention_kernel(const PaParams P) {
         qk *= up;
         if (P.k_scale) qk *= P.k_scale[kvh];
       }
+      // a factor above zero keeps the order of the scores (and -inf times it is -inf)
+      if (qk < 0.0f) {
+        qk = -qk;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) qa[i][x] ^= 0x80008000u;
+      }
+      qk = fmaxf(qk, 1e-37f);
     }
 
     float o[kT][4];
@@ -386,29 +431,31 @@ paged_attention_kernel(const PaParams P) {
     for (int i = 0; i < kT; ++i)
 #pragma unroll
       for (int x = 0; x < 4; ++x) o[i][x] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
+    float m = -INFINITY;
+    float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // sums of P, a product with a column of ones
 
-    for (int base = lo + warp * kStep; base < hi; base += S::kUnit) {
-      const int stage = used % S::kStages;
-      if (!wait_full(&full_s[warp][stage], (used / S::kStages) & 1, gave_up ? 0 : P.wait_ns)) {
+    for (int base = lo + warp * S::kStep; base < hi; base += S::kUnit) {
+      if (!wait_full(&full_s[warp][stage], phase, gave_up ? 0 : P.wait_ns)) {
         gave_up = true;  // nothing more is issued: the stage's barrier may still be open
         more = false;
         if (lane == 0 && P.status) atomicOr(P.status, MC_KV_WAIT);
       }
-      const uint32_t live = live_s[warp][stage] >> (kPart * c) & 0xffu;
-      const uint8_t* ks = ring + stage * S::kStage + (hr >> 1) * S::kPartBytes + (hr & 1) * S::kRow + 16 * c;
-      const uint8_t* vs = ring + stage * S::kStage + S::kHalf + c * S::kPartBytes +
-                          (F8 && D == 64 ? 8 : 16) * hr;
-      // ---- scores of 32 keys for 8 heads; key 8 c + 4 z + 2 j + x in t[z][2 j + x]
-      float t[2][4];
+      const uint32_t live = live_s[warp][stage] >> (S::kPart * c) & kAll;
+      const uint8_t* k0 = ring + stage * S::kStage + k_at;
+      const uint8_t* k1 = k0 + k_flip;
+      const uint8_t* v0 = ring + stage * S::kStage + S::kHalf + v_at;
+      const uint8_t* v1 = v0 + v_flip;
+      // ---- scores for 8 heads; key kPart c + 4 z + 2 j + x in t[z][2 j + x]
+      float t[kZ][4];
 #pragma unroll
-      for (int z = 0; z < 2; ++z)
+      for (int z = 0; z < kZ; ++z)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
           for (int i = 0; i < kKLoads; ++i) {
-            const uint4 w = *reinterpret_cast<const uint4*>(ks + (4 * z + 2 * j) * S::kRow + 64 * i);
+            const uint4 w = *reinterpret_cast<const uint4*>(
+                (i & 1 ? k1 : k0) + (4 * z + 2 * j) * S::kRow + 128 * (i >> 1));
             if (!F8) {
               mma16816<false>(s, qa[2 * i][0], 0u, qa[2 * i][1], 0u, w.x, w.y);
               mma16816<false>(s, qa[2 * i + 1][0], 0u, qa[2 * i + 1][1], 0u, w.z, w.w);
@@ -421,24 +468,27 @@ paged_attention_kernel(const PaParams P) {
               }
             }
           }
-          t[z][2 * j] = s[0] * qk;
-          t[z][2 * j + 1] = s[1] * qk;
+          t[z][2 * j] = s[0];
+          t[z][2 * j + 1] = s[1];
         }
       // ---- running maximum and sum of head lane/4
-      if (live != 0xffu) {
+      if (live != kAll) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 4 * kZ; ++i)
           if (!(live >> i & 1u)) t[i / 4][i % 4] = -INFINITY;
       }
-      float top = fmaxf(fmaxf(fmaxf(t[0][0], t[0][1]), fmaxf(t[0][2], t[0][3])),
-                        fmaxf(fmaxf(t[1][0], t[1][1]), fmaxf(t[1][2], t[1][3])));
+      float top = fmaxf(fmaxf(t[0][0], t[0][1]), fmaxf(t[0][2], t[0][3]));
+#pragma unroll
+      for (int z = 1; z < kZ; ++z)
+        top = fmaxf(top, fmaxf(fmaxf(t[z][0], t[z][1]), fmaxf(t[z][2], t[z][3])));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float m_new = fmaxf(m, top);
+      const float m_new = fmaxf(m, top * qk);
       const float m_use = m_new == -INFINITY ? 0.0f : m_new;
       if (__any_sync(0xffffffffu, m_new != m)) {
         const float a = ex2(m - m_use);
-        l *= a;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) l4[x] *= a;
 #pragma unroll
         for (int i = 0; i < kT; ++i)
 #pragma unroll
@@ -446,13 +496,10 @@ paged_attention_kernel(const PaParams P) {
         m = m_new;
       }
 #pragma unroll
-      for (int z = 0; z < 2; ++z) {
+      for (int z = 0; z < kZ; ++z) {
         float p[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[i] = ex2(t[z][i] - m_use);
-          l += p[i];
-        }
+        for (int i = 0; i < 4; ++i) p[i] = ex2(__fmaf_rn(t[z][i], qk, -m_use));
         const uint32_t h0 = pack2<F8>(p[0], p[1]), h1 = pack2<F8>(p[2], p[3]);
         const float2 g0 = unpack2<F8>(h0), g1 = unpack2<F8>(h1);
         const uint32_t w0 = pack2<F8>(p[0] - g0.x, p[1] - g0.y);
@@ -460,8 +507,10 @@ paged_attention_kernel(const PaParams P) {
         uint32_t v[4][kVWords];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint8_t* vr = vs + (4 * z + i) * S::kRow;
-          if (F8 && D == 64) {
+          // an odd key's chunks lie in the other half of the line
+          const uint8_t* vr = kHalfChunk ? (i & 1 ? v1 : v0) + 256 * z + 128 * (i >> 1)
+                                         : (i & 1 ? v1 : v0) + (4 * z + i) * S::kRow;
+          if (kHalfChunk) {
             const uint2 u = *reinterpret_cast<const uint2*>(vr);
             v[i][0] = u.x;
             v[i][1] = u.y;
@@ -476,11 +525,13 @@ paged_attention_kernel(const PaParams P) {
             }
           }
           // a key left out has a weight of zero, but what lies in its place may be NaN
-          if (live != 0xffu && !(live >> (4 * z + i) & 1u)) {
+          if (live != kAll && !(live >> (4 * z + i) & 1u)) {
 #pragma unroll
             for (int n = 0; n < kVWords; ++n) v[i][n] = 0u;
           }
         }
+        constexpr uint32_t kOnes = F8 ? 0x3c003c00u : 0x3f803f80u;
+        mma16816<F8>(l4, h0, w0, h1, w1, kOnes, kOnes);
         // ---- o += P V: rows 0-7 the high parts, rows 8-15 the low parts
         if (!F8) {
 #pragma unroll
@@ -504,14 +555,16 @@ paged_attention_kernel(const PaParams P) {
           }
         }
       }
-      ++used;
+      if (++stage == S::kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
       __syncwarp();  // every lane has read the stage
       if (more) issue();
     }
 
     // ---- the warps' results of this piece
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    float l = l4[0] + l4[2];
     if (gave_up) l = __uint_as_float(0x7fc00000u);  // what did not arrive makes the result NaN
     __syncthreads();  // the piece before is done with the shared arrays
     if (c == 0) {
@@ -528,15 +581,6 @@ paged_attention_kernel(const PaParams P) {
     __syncthreads();
     const bool begins = piece.unit == 0, ends = piece.unit + piece.units == piece.n;
     float* part = P.parts + part_floats(D) * (2 * (size_t)cta + (begins ? 1 : 0));
-    auto finish = [&](int h, int d, float mx, float sum, float val) {
-      if (h >= heads) return;
-      const float vscale = F8 && P.v_scale ? P.v_scale[kvh] : 1.0f;
-      const float r = sum == 0.0f ? 0.0f : __fdiv_rn(val, sum) * vscale;
-      P.out[(size_t)row * P.out_stride + (size_t)(head0 + h) * D + d] = mc_f32_to_bf16(r);
-      if (P.lse && d == 0)
-        P.lse[(size_t)row * P.H + head0 + h] =
-            sum == 0.0f ? -INFINITY : __fmaf_rn(mx, kLn2, logf(sum));
-    };
     for (int i = tid; i < kHeads * D; i += S::kThreads) {
       const int h = i / D, d = i % D;
       float mx = m_s[0][h];
@@ -551,7 +595,7 @@ paged_attention_kernel(const PaParams P) {
         val = __fmaf_rn(a, o_s[(w * kHeads + h) * S::kORow + d], val);
       }
       if (begins && ends) {
-        finish(h, d, mx, sum, val);
+        if (h < heads) finish(row, head0 + h, kvh, d, mx, sum, val);
       } else {
         part[i] = val;
         if (d == 0) {
@@ -565,16 +609,16 @@ paged_attention_kernel(const PaParams P) {
     const long long first_unit = u_end - piece.left - piece.unit;
     const int first_cta = begins ? cta : ps_owner(first_unit, U, G);
     const int last_cta = ends ? cta : ps_owner(first_unit + piece.n - 1, U, G);
-    __threadfence();
     __syncthreads();
     if (tid == 0) {
+      __threadfence();  // this CTA's part, written before the barrier
       const uint32_t done = atomicAdd(P.counters + first_cta, 1u);
       last_s = done == (uint32_t)(last_cta - first_cta);
       if (last_s) P.counters[first_cta] = 0;
+      __threadfence();
     }
     __syncthreads();
     if (!last_s) continue;
-    __threadfence();
     auto part_of = [&](int x) {
       return P.parts + part_floats(D) * (2 * (size_t)x + (x == first_cta ? 1 : 0));
     };
@@ -599,8 +643,7 @@ paged_attention_kernel(const PaParams P) {
       const int h = 4 * i / D;
       float mx = -INFINITY, sum = 0.0f;
 #pragma unroll
-      for (int w = 0; w < S::kWarps; ++w)
-        fold(mx, sum, m_s[w][h], l_s[w][h]);
+      for (int y = 0; y < S::kWarps; ++y) fold(mx, sum, m_s[y][h], l_s[y][h]);
       const float use = mx == -INFINITY ? 0.0f : mx;
       float4 val = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       for (int x0 = first_cta; x0 <= last_cta; x0 += 8) {
@@ -626,10 +669,10 @@ paged_attention_kernel(const PaParams P) {
         }
       }
       const int d = 4 * i % D;
-      finish(h, d, mx, sum, val.x);
-      finish(h, d + 1, mx, sum, val.y);
-      finish(h, d + 2, mx, sum, val.z);
-      finish(h, d + 3, mx, sum, val.w);
+      finish(row, head0 + h, kvh, d, mx, sum, val.x);
+      finish(row, head0 + h, kvh, d + 1, mx, sum, val.y);
+      finish(row, head0 + h, kvh, d + 2, mx, sum, val.z);
+      finish(row, head0 + h, kvh, d + 3, mx, sum, val.w);
     }
   } while (ps_next(piece, P.items, P.rows, units_of));
   if (gave_up) {  // copies still on their way end before the shared memory goes
@@ -643,7 +686,7 @@ int launch_attention(mc_ctx* ctx, const PaParams& P) {
   using S = Shape<D, F8>;
   auto fn = paged_attention_kernel<D, F8>;
   MC_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
-  long long g = (long long)ctx->num_sms * kPerSm;
+  long long g = (long long)ctx->num_sms * S::kPerSm;
   const long long most =
       (((long long)P.width * P.block_size + S::kUnit - 1) / S::kUnit) * P.rows * P.items;
   if (g > most) g = most;
@@ -701,9 +744,9 @@ extern "C" int mc_paged_attention(mc_ctx* ctx, const uint16_t* q, size_t q_strid
   MC_CUDA(dev.error());
   const int group = n_heads / n_kv_heads, subs = (group + kHeads - 1) / kHeads;
   const PaParams P{q, q_stride, n_rows, n_heads, n_kv_heads, group, subs, n_kv_heads * subs,
-                   k_cache, v_cache, num_blocks, block_size, block_stride, k_scale, v_scale,
-                   block_table, n_req, table_width, kv_lens, row_req, window, scale * kLog2e, out,
-                   out_stride, lse, static_cast<uint32_t*>(workspace),
+                   k_cache, v_cache, num_blocks, block_size, (uint32_t)(block_stride / head_dim),
+                   ps_div_of(block_size), k_scale, v_scale, block_table, n_req, table_width, kv_lens, row_req, window, scale * kLog2e,
+                   out, out_stride, lse, static_cast<uint32_t*>(workspace),
                    reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes), status,
                    mc_wait_limit(ctx, 1000000000ull)};
   const bool f8 = kv_dtype == MC_DTYPE_E4M3;

@@ -18,6 +18,31 @@
 #define PS_HD inline
 #endif
 
+// n / d for 0 <= n < 2^31 by one multiplication: with l = ceil(log2 d) and
+// m = floor(2^(31+l) / d) + 1 < 2^32 + 1, n m / 2^(31+l) exceeds n / d by less
+// than n / 2^(31+l) < 1 / d (d = 1: the number itself).
+struct PsDiv {
+  uint32_t mul;
+  int shift;  // -1: d = 1
+};
+inline PsDiv ps_div_of(int d) {
+  PsDiv r{0, -1};
+  if (d == 1) return r;
+  int l = 0;
+  while ((1ll << l) < d) ++l;
+  r.mul = (uint32_t)(((1ull << (31 + l)) / (unsigned)d) + 1);
+  r.shift = l - 1;
+  return r;
+}
+PS_HD int ps_div(int n, PsDiv d) {
+  if (d.shift < 0) return n;
+#ifdef __CUDA_ARCH__
+  return (int)(__umulhi((uint32_t)n, d.mul) >> d.shift);
+#else
+  return (int)(((uint64_t)(uint32_t)n * d.mul) >> 32 >> d.shift);
+#endif
+}
+
 // Keys of a row: [low, len).
 struct PsRow {
   int low, len;

@@ -77,9 +77,25 @@ static void run(const std::vector<int>& lens, long long capacity, int window, in
   }
 }
 
+static void divisions(std::mt19937& g) {
+  std::vector<int> ds{1, 2, 3, 5, 7, 16, 20, 24, 1000, 65535, 65536, 65537, 0x3fffffff, 0x40000000, 0x40000001, 0x7ffffffe, 0x7fffffff};
+  for (int i = 0; i < 300; ++i) ds.push_back((int)(g() >> (1 + g() % 30)) | 1), ds.push_back((int)(g() >> (1 + g() % 30)) + 1);
+  for (int d : ds) {
+    if (d < 1) continue;
+    const PsDiv v = ps_div_of(d);
+    CHECK(d == 1 || (v.shift >= 0 && v.shift < 32));
+    for (int i = 0; i < 2000; ++i) {
+      const int k = (int)(g() >> 1) / d;  // multiples of d and their neighbours, and anything
+      for (long long n : {(long long)k * d - 1, (long long)k * d, (long long)k * d + 1, (long long)(g() >> 1), 0x7fffffffll - i})
+        if (n >= 0 && n <= 0x7fffffff) CHECK(ps_div((int)n, v) == n / d);
+    }
+  }
+}
+
 int main() {
   std::mt19937 g(7);
   auto pick = [&](int lo, int hi) { return std::uniform_int_distribution<int>(lo, hi)(g); };
+  divisions(g);
   run({0}, 16, 0, 1, 444, 64);
   run({1}, 16, 0, 8, 444, 64);
   run({131072}, 131072, 0, 8, 444, 64);

@@ -89,8 +89,8 @@ REFUSED = [
     ("mc_qk_norm_rope", dict(q_out=0x1000010), "overlaps q"),
     ("mc_qk_norm_rope", dict(q_out=0x2000000), "overlaps k or v"),
     ("mc_qk_norm_rope", dict(eps=INF), "eps"),
-    ("mc_qk_norm_rope", dict(block_stride=8 * 16 * 64 - 8), "block stride"),
-    ("mc_qk_norm_rope", dict(block_stride=8 * 16 * 64 + 4), "16 bytes"),
+    ("mc_qk_norm_rope", dict(block_stride=8 * 16 * 64 - 64), "block stride"),
+    ("mc_qk_norm_rope", dict(block_stride=8 * 16 * 64 + 8), "multiple of head_dim"),
     ("mc_qk_norm_rope", dict(k_cache=0x10008), "16-byte"),
     ("mc_qk_norm_rope", dict(k_scale=0x100), "e4m3"),
     ("mc_paged_attention", dict(n_rows=-1), "n_rows"),
@@ -108,6 +108,7 @@ REFUSED = [
     ("mc_paged_attention", dict(ws_bytes=1000), "workspace"),
     ("mc_paged_attention", dict(workspace=0x3000008), "workspace"),
     ("mc_paged_attention", dict(num_blocks=0), "blocks"),
+    ("mc_paged_attention", dict(num_blocks=1 << 25), "2^32"),
     ("mc_logits_process", dict(dtype=_lib.DTYPE_E4M3), "dtype"),
     ("mc_logits_process", dict(vocab=0), "vocab"),
     ("mc_logits_process", dict(batch=65536), "batch"),
@@ -138,7 +139,7 @@ def test_refusals(lib, name, changed, words):
     ("mc_qk_norm_rope", dict(v=None, q_norm_w=None, k_norm_w=None, slots=None)),
     ("mc_qk_norm_rope", dict(rot_dim=0, positions=None, turns=None)),
     ("mc_qk_norm_rope", dict(kv_dtype=_lib.DTYPE_E4M3, k_scale=0x600, v_scale=0x700)),
-    ("mc_qk_norm_rope", dict(num_blocks=1, block_size=1, block_stride=512)),
+    ("mc_qk_norm_rope", dict(num_blocks=1, block_size=1, block_stride=0)),
     ("mc_paged_attention", dict(row_req=0x500, n_rows=1000)),
     ("mc_paged_attention", dict(n_heads=8)),
     ("mc_logits_process", dict(out=0x1000000)),                              # in place
