@@ -324,7 +324,8 @@ int mc_sample_mark(mc_ctx* ctx, const uint32_t* tok, uint32_t* seen, int vocab,
  * >= n_kv_heads * block_size * head_dim and a multiple of head_dim, so K and
  * V pages may alternate in one allocation). block_size is any positive
  * number; head_dim 64 or 128; kv_dtype MC_DTYPE_BF16, or MC_DTYPE_E4M3 with
- * optional scales f32[n_kv_heads] (stored = value / scale, saturating; read =
+ * optional scales f32[n_kv_heads], positive and normal (stored = value /
+ * scale, saturating; read =
  * stored * scale). With num_blocks = 1 and block_size = max_seq it is the
  * cache mc_proj3_gemv_scatter writes. Slot s is row s % block_size of page
  * s / block_size; all ones means "not written". A request's block table row

@@ -50,7 +50,7 @@ template <bool F32, bool VEC>
 __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const RulesParams P) {
   mc_pdl_launch_dependents();
   mc_pdl_wait();
-  __shared__ float bias_s[kTokens];
+  __shared__ __align__(16) float bias_s[kTokens];
   __shared__ unsigned long long key_s[kThreads / 32];
   const int b = blockIdx.y, tid = threadIdx.x;
   const int i0 = blockIdx.x * kTokens + tid * 8;
@@ -60,6 +60,7 @@ __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const RulesParam
 
   float v[8];
   uint32_t seen = 0, allowed = 0xff;
+  bool counted = false;
   uint16_t cnt[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   {
     const uint16_t* x16 = static_cast<const uint16_t*>(P.logits) + (size_t)b * P.stride + i0;
@@ -90,7 +91,9 @@ __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const RulesParam
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int i = 0; i < 8; ++i) cnt[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+        counted = (u.x | u.y | u.z | u.w) != 0;
       } else {
+        counted = true;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           if (i < n) cnt[i] = c[i];
@@ -106,57 +109,74 @@ __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const RulesParam
     }
   }
 
+  const float rep = P.rep ? P.rep[b] : 1.0f;
+  const float freq = P.freq ? P.freq[b] : 0.0f, pres = P.pres ? P.pres[b] : 0.0f;
+
   // ---- biases of this CTA's tokens
   bool biased = false;
   if (P.bias_start) {
-    int lo = min(max(P.bias_start[b], 0), P.n_bias);
-    int hi = min(max(P.bias_start[b + 1], lo), P.n_bias);
+    const int start = min(max(P.bias_start[b], 0), P.n_bias);
+    const int end = min(max(P.bias_start[b + 1], start), P.n_bias);
     const uint32_t first = blockIdx.x * kTokens, last = first + kTokens;
-    if (hi > lo) {
+    if (end > start) {
       biased = true;
 #pragma unroll
       for (int i = 0; i < 8; ++i) bias_s[tid + i * kThreads] = 0.0f;
-      if (hi - lo > 4 * kThreads) {
+      int lo = start, hi = end;
+      if (end - start > 4 * kThreads) {
         // probes at every `step`-th entry bound the part with ids in [first, last)
-        const int step = (hi - lo + kThreads - 1) / kThreads;
-        const int at = lo + tid * step;
-        const uint32_t id = at < hi ? P.bias_ids[at] : 0xffffffffu;
-        const int below = __syncthreads_count(at < hi && id < first);
-        const int before = __syncthreads_count(at < hi && id < last);
-        const int base = lo;
-        lo = base + max(below - 1, 0) * step;
-        hi = min(hi, base + before * step);
+        const int step = (end - start + kThreads - 1) / kThreads;
+        const int at = start + tid * step;
+        const uint32_t id = at < end ? P.bias_ids[at] : 0xffffffffu;
+        const int below = __syncthreads_count(at < end && id < first);
+        const int before = __syncthreads_count(at < end && id < last);
+        lo = start + max(below - 1, 0) * step;
+        hi = min(end, start + before * step);
       }
       __syncthreads();
-      const int start = min(max(P.bias_start[b], 0), P.n_bias);
       for (int j = lo + tid; j < hi; j += kThreads) {
         const uint32_t id = P.bias_ids[j];
-        if (id < first || id >= last || (j > start && P.bias_ids[j - 1] == id)) continue;
+        const uint32_t back = P.bias_ids[max(j - 1, start)], next = P.bias_ids[min(j + 1, end - 1)];
         float sum = P.bias_vals[j];
-        const int end = min(max(P.bias_start[b + 1], start), P.n_bias);
-        for (int e = j + 1; e < end && P.bias_ids[e] == id; ++e)
-          sum = __fadd_rn(sum, P.bias_vals[e]);
+        if (id < first || id >= last || (j > start && back == id)) continue;
+        if (j + 1 < end && next == id)
+          for (int e = j + 1; e < end && P.bias_ids[e] == id; ++e)
+            sum = __fadd_rn(sum, P.bias_vals[e]);
         bias_s[id - first] = sum;
       }
       __syncthreads();
     }
   }
 
-  const float rep = P.rep ? P.rep[b] : 1.0f;
-  const float freq = P.freq ? P.freq[b] : 0.0f, pres = P.pres ? P.pres[b] : 0.0f;
-  unsigned long long best = 0;
+  if (seen) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float x = v[i];
-    if (seen >> i & 1) x = x > 0.0f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-    if (cnt[i]) x = __fadd_rn(__fadd_rn(x, -__fmul_rn(freq, (float)cnt[i])), -pres);
-    if (biased) x = __fadd_rn(x, bias_s[tid * 8 + i]);
-    if (!(allowed >> i & 1)) x = -INFINITY;
-    if (!F32) x = mc_round_bf16(x);
-    v[i] = x;
-    if (P.keys && i < n && x == x) {
-      const unsigned long long k = mc_argmax_key(x, (uint32_t)(i0 + i));
-      best = k > best ? k : best;
+    for (int i = 0; i < 8; ++i)
+      if (seen >> i & 1) v[i] = v[i] > 0.0f ? __fdiv_rn(v[i], rep) : __fmul_rn(v[i], rep);
+  }
+  if (counted) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (cnt[i]) v[i] = __fadd_rn(__fadd_rn(v[i], -__fmul_rn(freq, (float)cnt[i])), -pres);
+  }
+  if (biased) {
+    const float4 u = reinterpret_cast<const float4*>(bias_s)[2 * tid];
+    const float4 x = reinterpret_cast<const float4*>(bias_s)[2 * tid + 1];
+    const float add[8] = {u.x, u.y, u.z, u.w, x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fadd_rn(v[i], add[i]);
+  }
+  if (allowed != 0xff) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (!(allowed >> i & 1)) v[i] = -INFINITY;
+  }
+  uint32_t packed[4];
+  if (!F32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(packed[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
+      v[2 * i] = __uint_as_float(packed[i] << 16);
+      v[2 * i + 1] = __uint_as_float(packed[i] & 0xffff0000u);
     }
   }
   uint16_t* o16 = static_cast<uint16_t*>(P.out) + (size_t)b * P.out_stride + i0;
@@ -165,11 +185,7 @@ __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const RulesParam
     reinterpret_cast<float4*>(o32)[0] = make_float4(v[0], v[1], v[2], v[3]);
     reinterpret_cast<float4*>(o32)[1] = make_float4(v[4], v[5], v[6], v[7]);
   } else if (full) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w[i] = (__float_as_uint(v[2 * i]) >> 16) | (__float_as_uint(v[2 * i + 1]) & 0xffff0000u);
-    *reinterpret_cast<uint4*>(o16) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(o16) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -179,14 +195,28 @@ __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const RulesParam
     }
   }
   if (!P.keys) return;
+  // ---- the greedy key: the thread's largest value, the warp's, and the lowest index that has it
+  float top = -INFINITY;
 #pragma unroll
-  for (int m = 16; m >= 1; m >>= 1) {
-    const unsigned long long o = __shfl_xor_sync(0xffffffffu, best, m);
-    best = o > best ? o : best;
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, i < n ? v[i] : -INFINITY);  // NaN never wins
+  bool any = top != -INFINITY;
+  if (!any) {  // nothing, NaN, or -inf, which is a value too
+#pragma unroll
+    for (int i = 0; i < 8; ++i) any |= i < n && v[i] == v[i];
   }
-  if ((tid & 31) == 0) key_s[tid >> 5] = best;
+  const uint32_t mine = any ? mc_fkey(top) : 0u;
+  const uint32_t most = __reduce_max_sync(0xffffffffu, mine);
+  uint32_t at = 0xffffffffu;
+  if (any && mine == most) {
+#pragma unroll
+    for (int i = 7; i >= 0; --i)
+      if (i < n && v[i] == top) at = (uint32_t)(i0 + i);
+  }
+  at = __reduce_min_sync(0xffffffffu, at);
+  if ((tid & 31) == 0) key_s[tid >> 5] = most ? (unsigned long long)most << 32 | (uint32_t)~at : 0;
   __syncthreads();
   if (tid == 0) {
+    unsigned long long best = key_s[0];
 #pragma unroll
     for (int w = 1; w < kThreads / 32; ++w) best = key_s[w] > best ? key_s[w] : best;
     if (best) atomicMax(P.keys + b, best);

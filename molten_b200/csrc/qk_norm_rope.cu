@@ -15,11 +15,12 @@
 // position, and sincospi of the signed remainder.
 //
 // What bounds it: bytes (each row read once, written once), and latency at a
-// few tokens. A CTA takes one token: its threads first have the row loads in
-// flight (16 bytes a lane, head_dim/8 lanes a row), then compute the token's
-// cosines and sines once into shared memory for all its heads, then
-// normalise (a shuffle reduction inside the row's lanes) and rotate (the
-// partner 16 bytes come by shuffle).
+// few tokens. A thread holds 8 elements of one head row, the two groups of 4
+// that rotate into each other (so no pair crosses threads), for every token of
+// the CTA's batch: its gains, addresses and role stay in registers. A batch's
+// cosines, sines and cache rows are computed once into shared memory by all
+// threads together. Few tokens: a CTA each; many: up to 8 a CTA, 4 tokens'
+// loads in flight a thread.
 #include <cuda_fp8.h>
 #include <math.h>
 
@@ -28,13 +29,16 @@
 namespace {
 
 constexpr int kMaxThreads = 512;
+constexpr int kBatch = 8;   // most tokens of a CTA
+constexpr int kFlight = 4;  // tokens whose loads are in flight together
 
 struct RopeParams {
   const uint16_t* q;
   const uint16_t* k;
   const uint16_t* v;  // null: V is not written
   size_t q_stride, k_stride, v_stride;
-  int H, K, rows;  // rows = H + K (+ K with v)
+  int tokens, batch;      // tokens of a CTA: batch (1 to kBatch)
+  int H, K, rows, group;  // rows = H + K (+ K with v), `group` of them a CTA
   const uint16_t* qw;  // null: no norm
   const uint16_t* kw;
   float eps;
@@ -46,150 +50,186 @@ struct RopeParams {
   const unsigned long long* slots;  // null: token t goes to slot t
   void* kc;
   void* vc;
-  int num_blocks, block_size;
-  size_t block_stride;
+  uint32_t n_slots, page_rows, block_size;
   const float* k_scale;
   const float* v_scale;
   uint32_t* status;
 };
 
-__device__ __forceinline__ void unpack8(const uint4& u, float* f) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = mc_bf16_to_f32((uint16_t)(w[i >> 1] >> (16 * (i & 1))));
+__device__ __forceinline__ void unpack4(const uint2& u, float* f) {
+  f[0] = __uint_as_float(u.x << 16);
+  f[1] = __uint_as_float(u.x & 0xffff0000u);
+  f[2] = __uint_as_float(u.y << 16);
+  f[3] = __uint_as_float(u.y & 0xffff0000u);
 }
 
-__device__ __forceinline__ uint4 pack8(const float* f) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] = (uint32_t)mc_f32_to_bf16(f[2 * i]) | ((uint32_t)mc_f32_to_bf16(f[2 * i + 1]) << 16);
-  return make_uint4(w[0], w[1], w[2], w[3]);
+__device__ __forceinline__ uint2 pack4(const float* f) {
+  uint2 r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r.x) : "f"(f[1]), "f"(f[0]));
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r.y) : "f"(f[3]), "f"(f[2]));
+  return r;
 }
 
-__device__ __forceinline__ uint2 pack8_e4m3(const float* f) {
-  uint32_t w[2] = {0, 0};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __nv_fp8x2_storage_t b =
-        __nv_cvt_float2_to_fp8x2(make_float2(f[2 * i], f[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-    w[i >> 1] |= (uint32_t)b << (16 * (i & 1));
-  }
-  return make_uint2(w[0], w[1]);
+__device__ __forceinline__ uint32_t pack4_e4m3(const float* f) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3);
+  return lo | hi << 16;
 }
 
 // D: head_dim; F8: e4m3 cache.
 template <int D, bool F8>
 __global__ void __launch_bounds__(kMaxThreads) qk_norm_rope_kernel(const RopeParams P) {
-  constexpr int L = D / 8;  // lanes of a row
+  constexpr int L = D / 8;  // threads of a row
+  __shared__ float2 cs[kBatch][D / 2];
+  __shared__ uint32_t row_s[kBatch];  // the token's row of head 0 in the cache, all ones: none
+  const int tid = threadIdx.x, c = tid % L;
+  const int half = P.rot / 2, turned = P.rot / 8;  // threads of a row that rotate
+  const int t0 = blockIdx.x * P.batch, n = min(P.batch, P.tokens - t0);
+
+  // ---- this thread's row and its two groups of 4 elements
+  const int r = blockIdx.y * P.group + tid / L;
+  const bool in = r < P.rows && tid / L < P.group;
+  const bool is_q = r < P.H, is_k = !is_q && r < P.H + P.K;
+  const int h = is_q ? r : is_k ? r - P.H : r - P.H - P.K;
+  const bool turns_here = (is_q || is_k) && c < turned;
+  int a = 2 * c, b = 2 * c + 1;  // groups
+  if (!P.interleaved && c < turned) {
+    a = c;
+    b = c + turned;
+  }
+  const uint16_t* src = is_q ? P.q : is_k ? P.k : P.v;
+  const size_t stride = is_q ? P.q_stride : is_k ? P.k_stride : P.v_stride;
+  src += (size_t)t0 * stride + (size_t)h * D;
+  const uint16_t* w = is_q ? P.qw : is_k ? P.kw : nullptr;
   mc_pdl_launch_dependents();
   mc_pdl_wait();
-  __shared__ float2 cs[D / 2];
-  const int t = blockIdx.x;
-  const int lane = threadIdx.x & 31, c = lane % L;
-  const int half = P.rot / 2, hc = P.rot / 16;  // 16-byte chunks of half the rotated part
-  const int per_pass = blockDim.x / L;
-  const unsigned long long slot = P.slots ? P.slots[t] : (unsigned long long)t;
-  const unsigned long long n_slots = (unsigned long long)P.num_blocks * P.block_size;
-  const bool store = slot < n_slots;
-  if (!store && slot != MC_KV_SLOT_NONE && threadIdx.x == 0 && P.status)
-    atomicOr(P.status, MC_KV_BAD_SLOT);
-  const size_t page = store ? (size_t)(slot / P.block_size) * P.block_stride : 0;
-  const int off = store ? (int)(slot % P.block_size) : 0;
 
-  // every thread runs every pass: the shuffles need whole warps
-  for (int r0 = 0; r0 < P.rows; r0 += per_pass) {
-    const int r = r0 + threadIdx.x / L;
-    const bool in = r < P.rows;
-    const bool is_q = r < P.H, is_k = !is_q && r < P.H + P.K;
-    const int h = is_q ? r : is_k ? r - P.H : r - P.H - P.K;
-    uint4 raw = make_uint4(0, 0, 0, 0), wraw = make_uint4(0, 0, 0, 0);
-    const uint16_t* w = is_q ? P.qw : is_k ? P.kw : nullptr;
-    if (in) {
-      const uint16_t* src = is_q   ? P.q + (size_t)t * P.q_stride
-                            : is_k ? P.k + (size_t)t * P.k_stride
-                                   : P.v + (size_t)t * P.v_stride;
-      raw = reinterpret_cast<const uint4*>(src + (size_t)h * D)[c];  // q_out may be q
-      if (w) wraw = __ldg(reinterpret_cast<const uint4*>(w) + c);
-    }
-    if (r0 == 0) {
-      for (int i = threadIdx.x; i < half; i += blockDim.x) {
-        const unsigned long long turn =
-            (unsigned long long)(long long)P.positions[t] * P.turns[i];
-        // signed fraction of a turn in [-1/2, 1/2), doubled: half turns
-        const float x = __ll2float_rn((long long)turn) * 1.0842021724855044e-19f;  // 2^-63
-        float s, co;
-        sincospif(x, &s, &co);
-        cs[i] = make_float2(co, s);
+  uint2 xa[kFlight], xb[kFlight];
+  auto load = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i)
+      if (in && t + i < n) {
+        // plain loads: q_out may be q
+        xa[i] = *reinterpret_cast<const uint2*>(src + (size_t)(t + i) * stride + 4 * a);
+        xb[i] = *reinterpret_cast<const uint2*>(src + (size_t)(t + i) * stride + 4 * b);
       }
-      __syncthreads();
+  };
+  load(0);
+  float ga[4], gb[4];
+  if (in && w) {
+    unpack4(__ldg(reinterpret_cast<const uint2*>(w) + a), ga);
+    unpack4(__ldg(reinterpret_cast<const uint2*>(w) + b), gb);
+  }
+  float scale = 1.0f;
+  if (F8 && in && !is_q) {
+    const float* s = is_k ? P.k_scale : P.v_scale;
+    if (s) scale = __fdiv_rn(1.0f, s[h]);
+  }
+  for (int i = tid; i < n * half; i += blockDim.x) {
+    const int t = i / half, f = i - t * half;
+    const unsigned long long turn =
+        (unsigned long long)(long long)P.positions[t0 + t] * P.turns[f];
+    // signed fraction of a turn in [-1/2, 1/2), doubled: half turns
+    const float x = __ll2float_rn((long long)turn) * 1.0842021724855044e-19f;  // 2^-63
+    float s, co;
+    sincospif(x, &s, &co);
+    cs[t][f] = make_float2(co, s);
+  }
+  if (tid < n) {
+    const unsigned long long slot = P.slots ? P.slots[t0 + tid] : (unsigned long long)(t0 + tid);
+    uint32_t row = 0xffffffffu;
+    if (slot < P.n_slots) {
+      const uint32_t page = (uint32_t)slot / P.block_size;
+      row = page * P.page_rows + ((uint32_t)slot - page * P.block_size);
+    } else if (slot != MC_KV_SLOT_NONE && P.status && blockIdx.y == 0) {
+      atomicOr(P.status, MC_KV_BAD_SLOT);
     }
-    float x[8];
-    unpack8(raw, x);
-    float ss = 0.0f;
+    row_s[tid] = row;
+  }
+  __syncthreads();
+
+  for (int t = 0; t < n; t += kFlight) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = __fmaf_rn(x[i], x[i], ss);
+    for (int i = 0; i < kFlight; ++i) {
+      if (t + i >= n) break;  // the same for the whole CTA
+      float x[4], y[4];
+      unpack4(xa[i], x);
+      unpack4(xb[i], y);
+      if (P.qw || P.kw) {
+        float ss = 0.0f;
 #pragma unroll
-    for (int m = 1; m < L; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-    if (w) {
-      const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fmaf_rn(ss, 1.0f / D, P.eps)));
-      float g[8];
-      unpack8(wraw, g);
+        for (int j = 0; j < 4; ++j) ss = __fmaf_rn(x[j], x[j], __fmaf_rn(y[j], y[j], ss));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * g[i];
-    }
-    // the other chunk of a half-split pair: c + hc or c - hc
-    const int pc = c < hc ? c + hc : c < 2 * hc ? c - hc : c;
-    float o[8];
+        for (int m = 1; m < L; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+        if (w) {
+          const float inv = rsqrtf(__fmaf_rn(ss, 1.0f / D, P.eps));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = __shfl_sync(0xffffffffu, x[i], (lane - c) + pc);
-    if (is_q || is_k) {
-      if (P.interleaved) {
-        if (c < 2 * hc) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 e = cs[c * 4 + i];
-            const float a = x[2 * i], b = x[2 * i + 1];
-            x[2 * i] = __fmaf_rn(a, e.x, -(b * e.y));
-            x[2 * i + 1] = __fmaf_rn(b, e.x, a * e.y);
+          for (int j = 0; j < 4; ++j) {
+            x[j] = x[j] * inv * ga[j];
+            y[j] = y[j] * inv * gb[j];
           }
         }
-      } else if (c < 2 * hc) {
-        const bool first = c < hc;
+      }
+      if (turns_here) {
+        if (P.interleaved) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 e = cs[(first ? c : c - hc) * 8 + i];
-          x[i] = first ? __fmaf_rn(x[i], e.x, -(o[i] * e.y)) : __fmaf_rn(x[i], e.x, o[i] * e.y);
+          for (int j = 0; j < 4; j += 2) {
+            const float2 e = cs[t + i][4 * c + j / 2], f = cs[t + i][4 * c + 2 + j / 2];
+            const float p = x[j], q = y[j];
+            x[j] = __fmaf_rn(p, e.x, -(x[j + 1] * e.y));
+            x[j + 1] = __fmaf_rn(x[j + 1], e.x, p * e.y);
+            y[j] = __fmaf_rn(q, f.x, -(y[j + 1] * f.y));
+            y[j + 1] = __fmaf_rn(y[j + 1], f.x, q * f.y);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 e = cs[t + i][4 * c + j];
+            const float p = x[j];
+            x[j] = __fmaf_rn(p, e.x, -(y[j] * e.y));
+            y[j] = __fmaf_rn(y[j], e.x, p * e.y);
+          }
+        }
+      }
+      if (!in) continue;
+      if (is_q) {
+        uint16_t* to = P.q_out + (size_t)(t0 + t + i) * P.q_out_stride + (size_t)h * D;
+        *reinterpret_cast<uint2*>(to + 4 * a) = pack4(x);
+        *reinterpret_cast<uint2*>(to + 4 * b) = pack4(y);
+      } else if (row_s[t + i] != 0xffffffffu) {
+        const size_t at = ((size_t)row_s[t + i] + (size_t)h * P.block_size) * D;
+        void* cache = is_k ? P.kc : P.vc;
+        if (F8) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[j] *= scale;
+            y[j] *= scale;
+          }
+          uint8_t* to = static_cast<uint8_t*>(cache) + at;
+          *reinterpret_cast<uint32_t*>(to + 4 * a) = pack4_e4m3(x);
+          *reinterpret_cast<uint32_t*>(to + 4 * b) = pack4_e4m3(y);
+        } else {
+          uint16_t* to = static_cast<uint16_t*>(cache) + at;
+          *reinterpret_cast<uint2*>(to + 4 * a) = pack4(x);
+          *reinterpret_cast<uint2*>(to + 4 * b) = pack4(y);
         }
       }
     }
-    if (!in) continue;
-    if (is_q) {
-      reinterpret_cast<uint4*>(P.q_out + (size_t)t * P.q_out_stride + (size_t)h * D)[c] = pack8(x);
-    } else if (store) {
-      const size_t at = page + ((size_t)h * P.block_size + off) * D + 8 * c;
-      void* cache = is_k ? P.kc : P.vc;
-      if (F8) {
-        const float* scale = is_k ? P.k_scale : P.v_scale;
-        if (scale) {
-          const float s = scale[h];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = __fdiv_rn(x[i], s);
-        }
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + at) = pack8_e4m3(x);
-      } else {
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(cache) + at) = pack8(x);
-      }
-    }
+    load(t + kFlight);
   }
 }
 
 template <int D, bool F8>
-int launch_rope(mc_ctx* ctx, const RopeParams& P, int n_tokens) {
-  int threads = ((P.rows * (D / 8) + 31) / 32) * 32;
-  if (threads > kMaxThreads) threads = kMaxThreads;
-  MC_CUDA(mc_launch_pdl(qk_norm_rope_kernel<D, F8>, dim3(n_tokens), dim3(threads), 0, ctx->stream,
-                        P));
+int launch_rope(mc_ctx* ctx, RopeParams& P) {
+  // rows of a token: even parts of at most kMaxThreads threads
+  const int most = kMaxThreads / (D / 8), parts = (P.rows + most - 1) / most;
+  P.group = (P.rows + parts - 1) / parts;
+  const int threads = (P.group * (D / 8) + 31) / 32 * 32;
+  // a CTA takes more tokens once every SM has some 4 of them
+  const long long some = 4ll * ctx->num_sms, batch = ((long long)P.tokens * parts + some - 1) / some;
+  P.batch = batch > kBatch ? kBatch : (int)batch;
+  const dim3 grid((unsigned)((P.tokens + P.batch - 1) / P.batch), (unsigned)parts);
+  MC_CUDA(mc_launch_pdl(qk_norm_rope_kernel<D, F8>, grid, dim3(threads), 0, ctx->stream, P));
   return mc_after_launch("qk_norm_rope_kernel");
 }
 
@@ -263,14 +303,13 @@ extern "C" int mc_qk_norm_rope(mc_ctx* ctx, const uint16_t* q, size_t q_stride, 
   MC_REQUIRE(ctx, "%s: null context", name);
   McDeviceGuard dev(ctx->device);
   MC_CUDA(dev.error());
-  const RopeParams P{q, k, v, q_stride, k_stride, v_stride, n_heads, n_kv_heads,
-                     n_heads + n_kv_heads * (v ? 2 : 1), q_norm_w, k_norm_w, eps, positions,
-                     reinterpret_cast<const unsigned long long*>(turns), rot_dim, interleaved,
-                     q_out, q_out_stride, reinterpret_cast<const unsigned long long*>(slots),
-                     k_cache, v_cache, num_blocks, block_size, block_stride, k_scale, v_scale,
-                     status};
+  RopeParams P{q, k, v, q_stride, k_stride, v_stride, n_tokens, 1, n_heads, n_kv_heads,
+               n_heads + n_kv_heads * (v ? 2 : 1), 0, q_norm_w, k_norm_w, eps, positions,
+               reinterpret_cast<const unsigned long long*>(turns), rot_dim, interleaved, q_out,
+               q_out_stride, reinterpret_cast<const unsigned long long*>(slots), k_cache, v_cache,
+               (uint32_t)num_blocks * (uint32_t)block_size, (uint32_t)(block_stride / head_dim),
+               (uint32_t)block_size, k_scale, v_scale, status};
   const bool f8 = kv_dtype == MC_DTYPE_E4M3;
-  if (head_dim == 64)
-    return f8 ? launch_rope<64, true>(ctx, P, n_tokens) : launch_rope<64, false>(ctx, P, n_tokens);
-  return f8 ? launch_rope<128, true>(ctx, P, n_tokens) : launch_rope<128, false>(ctx, P, n_tokens);
+  if (head_dim == 64) return f8 ? launch_rope<64, true>(ctx, P) : launch_rope<64, false>(ctx, P);
+  return f8 ? launch_rope<128, true>(ctx, P) : launch_rope<128, false>(ctx, P);
 }
