@@ -416,7 +416,7 @@ int mc_paged_attention(mc_ctx* ctx, const uint16_t* q, size_t q_stride, int n_ro
  * rows [batch][vocab] (dtype MC_DTYPE_BF16 or MC_DTYPE_F32, row strides in
  * elements) before argmax or mc_sample_draw. For token i of row b, in fp32:
  *   seen bit i (u32 bitmap [batch][ceil(vocab/32)]): v > 0 ? v / repetition[b]
- *     : v * repetition[b];
+ *     : v * repetition[b] (the quotient as a product with the reciprocal);
  *   counts[b][i] > 0 (u16): v - frequency[b] * count - presence[b];
  *   + the biases bias_vals[j] of the entries j in bias_start[b] ..
  *     bias_start[b + 1] (of n_bias) with bias_ids[j] = i; ids ascend within a

@@ -10,9 +10,12 @@
 // 64-bit greedy key of the head (largest value, ties to the lowest id, NaN
 // never), which mc_token_tail reads.
 //
-// What bounds it: bytes, 2 to 8 read and 2 or 4 written a token. A thread
-// takes 8 tokens: one 16-byte load of bf16 logits, one of counts, one byte of
-// each bitmap. A CTA takes 2048 tokens of one row. Biases are a short sorted
+// What bounds it: bytes (2 to 8 read and 2 or 4 written a token) and, with
+// every rule on, instructions, some 40 a token and lane. A thread takes 8
+// tokens: one 16-byte load of bf16 logits, one of counts, one byte of each
+// bitmap, the next span's on their way while it works on one (48 rows of
+// 128000 with all rules, in L2: 24 us without, 15 us). A CTA takes up to 4 spans of 2048 tokens of one row, so that a large
+// batch is one wave. Biases are a short sorted
 // list a row; each CTA looks through the part that can fall into its tokens
 // (256 probes narrow a long list) and the thread at the first of a run of
 // equal ids adds the run up into shared memory, so no order of atomics enters.
@@ -21,7 +24,9 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTokens = 8 * kThreads;
+constexpr int kSpan = 8 * kThreads;  // tokens a CTA takes at once
+constexpr int kSpans = 4;            // most spans of a CTA
+constexpr int kResident = 5;         // CTAs an SM holds at once
 
 struct RulesParams {
   const void* logits;
@@ -42,93 +47,127 @@ struct RulesParams {
   void* out;
   size_t out_stride;
   unsigned long long* keys;
+  int spans;
 };
 
-// F32: logits and output are float, else bf16. VEC: every row of every array
-// starts on 16 bytes, so a full group of 8 is loaded whole.
+// The 8 logits of one thread's group, as stored, with what the rules say about them.
+template <bool F32>
+struct Group {
+  uint32_t x[F32 ? 8 : 4];
+  uint32_t cnt[4];         // counts, two a word
+  uint32_t seen, allowed;  // a bit each
+};
+
+// Bits i .. i + 7 of a bitmap of `bytes` bytes (i from -7 on; bits outside are 0).
+__device__ __forceinline__ uint32_t bits8(const uint8_t* map, int i, int bytes) {
+  const int at = i >> 3, sh = i & 7;
+  uint32_t w = i >= 0 ? map[at] : 0u;
+  if (sh && at + 1 < bytes) w |= (uint32_t)map[at + 1] << 8;
+  return w >> sh & 0xffu;
+}
+
+// F32: logits and output are float, else bf16. VEC: the rows of logits, output
+// and counts all start equally far behind a 16-byte border (`shift` elements,
+// another number for each row of an odd vocabulary): groups of 8 begin at the
+// borders, and all but a row's first and last are loaded whole.
 template <bool F32, bool VEC>
-__global__ void __launch_bounds__(kThreads) logits_rules_kernel(const RulesParams P) {
+__global__ void __launch_bounds__(kThreads, kResident) logits_rules_kernel(const RulesParams P) {
   mc_pdl_launch_dependents();
   mc_pdl_wait();
-  __shared__ __align__(16) float bias_s[kTokens];
+  extern __shared__ __align__(16) float bias_s[];  // [spans * kSpan] where there are biases
   __shared__ unsigned long long key_s[kThreads / 32];
   const int b = blockIdx.y, tid = threadIdx.x;
-  const int i0 = blockIdx.x * kTokens + tid * 8;
-  const int n = min(8, P.vocab - i0);  // tokens of this thread (may be <= 0)
   const size_t words = ((size_t)P.vocab + 31) / 32;
-  const bool full = VEC && n == 8;
+  const uint16_t* x16 = static_cast<const uint16_t*>(P.logits) + (size_t)b * P.stride;
+  const float* x32 = static_cast<const float*>(P.logits) + (size_t)b * P.stride;
+  uint16_t* o16 = static_cast<uint16_t*>(P.out) + (size_t)b * P.out_stride;
+  float* o32 = static_cast<float*>(P.out) + (size_t)b * P.out_stride;
+  const uint16_t* counts = P.counts + (size_t)b * P.vocab;
+  const int shift = !VEC ? 0 : F32 ? (int)((uintptr_t)x32 / 4 % 4) : (int)((uintptr_t)x16 / 2 % 8);
+  const int first = blockIdx.x * P.spans * kSpan - shift;  // of this CTA; may be below 0
+  const uint8_t* seen =
+      P.seen ? reinterpret_cast<const uint8_t*>(P.seen + (size_t)b * words) : nullptr;
+  const uint8_t* allowed = nullptr;
+  if (P.allowed) {
+    const int row = P.allowed_row ? P.allowed_row[b] : b;
+    if (row >= 0 && row < P.n_allowed)
+      allowed = reinterpret_cast<const uint8_t*>(P.allowed + (size_t)row * words);
+  }
+  const float rep = P.rep ? P.rep[b] : 1.0f, inv = __fdiv_rn(1.0f, rep);  // as mc_sample_draw
+  const float freq = P.freq ? P.freq[b] : 0.0f, pres = P.pres ? P.pres[b] : 0.0f;
 
-  float v[8];
-  uint32_t seen = 0, allowed = 0xff;
-  bool counted = false;
-  uint16_t cnt[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  {
-    const uint16_t* x16 = static_cast<const uint16_t*>(P.logits) + (size_t)b * P.stride + i0;
-    const float* x32 = static_cast<const float*>(P.logits) + (size_t)b * P.stride + i0;
-    if (full && F32) {
+  auto load = [&](Group<F32>& w, int z) {
+    const int i1 = first + z * kSpan + tid * 8;
+    w.seen = 0;
+    w.allowed = 0xff;
 #pragma unroll
-      for (int z = 0; z < 2; ++z) {
-        const float4 u = reinterpret_cast<const float4*>(x32)[z];
-        v[4 * z] = u.x;
-        v[4 * z + 1] = u.y;
-        v[4 * z + 2] = u.z;
-        v[4 * z + 3] = u.w;
+    for (int i = 0; i < 4; ++i) w.cnt[i] = 0;
+    if (z >= P.spans || i1 >= P.vocab) return;
+    if (VEC && i1 >= 0 && i1 + 8 <= P.vocab) {
+#pragma unroll
+      for (int i = 0; i < (F32 ? 2 : 1); ++i) {
+        const uint4 u = F32 ? reinterpret_cast<const uint4*>(x32 + i1)[i]
+                            : *reinterpret_cast<const uint4*>(x16 + i1);
+        w.x[4 * i] = u.x;
+        w.x[4 * i + 1] = u.y;
+        w.x[4 * i + 2] = u.z;
+        w.x[4 * i + 3] = u.w;
       }
-    } else if (full) {
-      const uint4 u = *reinterpret_cast<const uint4*>(x16);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = mc_bf16_to_f32((uint16_t)(w[i >> 1] >> (16 * (i & 1))));
+      if (P.counts) {
+        uint2 c[2];  // rows of float logits begin on 8 bytes of counts
+        if (F32) {
+          c[0] = *reinterpret_cast<const uint2*>(counts + i1);
+          c[1] = *reinterpret_cast<const uint2*>(counts + i1 + 4);
+        } else {
+          const uint4 u = *reinterpret_cast<const uint4*>(counts + i1);
+          c[0] = make_uint2(u.x, u.y);
+          c[1] = make_uint2(u.z, u.w);
+        }
+        w.cnt[0] = c[0].x;
+        w.cnt[1] = c[0].y;
+        w.cnt[2] = c[1].x;
+        w.cnt[3] = c[1].y;
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[i] = i < n ? (F32 ? x32[i] : mc_bf16_to_f32(x16[i])) : -INFINITY;
-    }
-    if (P.counts) {
-      const uint16_t* c = P.counts + (size_t)b * P.vocab + i0;
-      if (full) {
-        const uint4 u = *reinterpret_cast<const uint4*>(c);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      for (int i = 0; i < (F32 ? 8 : 4); ++i) w.x[i] = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) cnt[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-        counted = (u.x | u.y | u.z | u.w) != 0;
-      } else {
-        counted = true;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < n) cnt[i] = c[i];
+      for (int i = 0; i < 8; ++i) {
+        if (i1 + i < 0 || i1 + i >= P.vocab) continue;
+        if (F32) w.x[i] = __float_as_uint(x32[i1 + i]);
+        else w.x[i / 2] |= (uint32_t)x16[i1 + i] << (16 * (i & 1));
+        if (P.counts) w.cnt[i / 2] |= (uint32_t)counts[i1 + i] << (16 * (i & 1));
       }
     }
-    if (n > 0) {
-      if (P.seen) seen = reinterpret_cast<const uint8_t*>(P.seen + (size_t)b * words)[i0 / 8];
-      if (P.allowed) {
-        const int row = P.allowed_row ? P.allowed_row[b] : b;
-        if (row >= 0 && row < P.n_allowed)
-          allowed = reinterpret_cast<const uint8_t*>(P.allowed + (size_t)row * words)[i0 / 8];
-      }
+    if (shift == 0) {
+      if (seen) w.seen = seen[i1 / 8];
+      if (allowed) w.allowed = allowed[i1 / 8];
+    } else {
+      if (seen) w.seen = bits8(seen, i1, (int)(4 * words));
+      if (allowed) w.allowed = bits8(allowed, i1, (int)(4 * words));
     }
-  }
+  };
 
-  const float rep = P.rep ? P.rep[b] : 1.0f;
-  const float freq = P.freq ? P.freq[b] : 0.0f, pres = P.pres ? P.pres[b] : 0.0f;
+  Group<F32> w, next;
+  load(w, 0);
 
   // ---- biases of this CTA's tokens
   bool biased = false;
   if (P.bias_start) {
     const int start = min(max(P.bias_start[b], 0), P.n_bias);
     const int end = min(max(P.bias_start[b + 1], start), P.n_bias);
-    const uint32_t first = blockIdx.x * kTokens, last = first + kTokens;
+    const uint32_t low = (uint32_t)max(first, 0), last = (uint32_t)(first + P.spans * kSpan);
     if (end > start) {
       biased = true;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) bias_s[tid + i * kThreads] = 0.0f;
+      for (int i = 0; i < 2 * P.spans; ++i)
+        reinterpret_cast<float4*>(bias_s)[tid + i * kThreads] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       int lo = start, hi = end;
       if (end - start > 4 * kThreads) {
-        // probes at every `step`-th entry bound the part with ids in [first, last)
+        // probes at every `step`-th entry bound the part with ids in [low, last)
         const int step = (end - start + kThreads - 1) / kThreads;
         const int at = start + tid * step;
         const uint32_t id = at < end ? P.bias_ids[at] : 0xffffffffu;
-        const int below = __syncthreads_count(at < end && id < first);
+        const int below = __syncthreads_count(at < end && id < low);
         const int before = __syncthreads_count(at < end && id < last);
         lo = start + max(below - 1, 0) * step;
         hi = min(end, start + before * step);
@@ -138,79 +177,110 @@ __global__ void __launch_bounds__(kThreads) logits_rules_kernel(const RulesParam
         const uint32_t id = P.bias_ids[j];
         const uint32_t back = P.bias_ids[max(j - 1, start)], next = P.bias_ids[min(j + 1, end - 1)];
         float sum = P.bias_vals[j];
-        if (id < first || id >= last || (j > start && back == id)) continue;
+        if (id < low || id >= last || (j > start && back == id)) continue;
         if (j + 1 < end && next == id)
           for (int e = j + 1; e < end && P.bias_ids[e] == id; ++e)
             sum = __fadd_rn(sum, P.bias_vals[e]);
-        bias_s[id - first] = sum;
+        bias_s[(int)id - first] = sum;
       }
       __syncthreads();
     }
   }
 
-  if (seen) {
+  float top = -INFINITY;  // this thread's largest value and the first group that has it (NaN
+  int best_z = -1;        // never wins)
+  auto apply = [&](const Group<F32>& w, int z) {
+    const int i1 = first + z * kSpan + tid * 8;
+    if (i1 >= P.vocab) return;
+    float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (seen >> i & 1) v[i] = v[i] > 0.0f ? __fdiv_rn(v[i], rep) : __fmul_rn(v[i], rep);
-  }
-  if (counted) {
+      v[i] = __uint_as_float(F32     ? w.x[i]
+                             : i & 1 ? w.x[i / 2] & 0xffff0000u
+                                     : w.x[i / 2] << 16);
+    if (w.seen) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (cnt[i]) v[i] = __fadd_rn(__fadd_rn(v[i], -__fmul_rn(freq, (float)cnt[i])), -pres);
-  }
-  if (biased) {
-    const float4 u = reinterpret_cast<const float4*>(bias_s)[2 * tid];
-    const float4 x = reinterpret_cast<const float4*>(bias_s)[2 * tid + 1];
-    const float add[8] = {u.x, u.y, u.z, u.w, x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __fadd_rn(v[i], add[i]);
-  }
-  if (allowed != 0xff) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (!(allowed >> i & 1)) v[i] = -INFINITY;
-  }
-  uint32_t packed[4];
-  if (!F32) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(packed[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
-      v[2 * i] = __uint_as_float(packed[i] << 16);
-      v[2 * i + 1] = __uint_as_float(packed[i] & 0xffff0000u);
+      for (int i = 0; i < 8; ++i) {
+        const float by = v[i] > 0.0f ? inv : rep;
+        v[i] = __fmul_rn(v[i], w.seen >> i & 1 ? by : 1.0f);
+      }
     }
-  }
-  uint16_t* o16 = static_cast<uint16_t*>(P.out) + (size_t)b * P.out_stride + i0;
-  float* o32 = static_cast<float*>(P.out) + (size_t)b * P.out_stride + i0;
-  if (full && F32) {
-    reinterpret_cast<float4*>(o32)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(o32)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else if (full) {
-    *reinterpret_cast<uint4*>(o16) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
-  } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i >= n) continue;
-      if (F32) o32[i] = v[i];
-      else o16[i] = (uint16_t)(__float_as_uint(v[i]) >> 16);
+    for (int i = 0; i < 8; i += 2) {
+      const uint32_t two = w.cnt[i / 2];
+      if (two == 0) continue;
+      const float c0 = (float)(two & 0xffffu), c1 = (float)(two >> 16);
+      if (two & 0xffffu) v[i] = __fadd_rn(__fadd_rn(v[i], -__fmul_rn(freq, c0)), -pres);
+      if (two >> 16) v[i + 1] = __fadd_rn(__fadd_rn(v[i + 1], -__fmul_rn(freq, c1)), -pres);
     }
+    if (biased) {
+      const float4* add = reinterpret_cast<const float4*>(bias_s + z * kSpan + tid * 8);
+      const float4 u = add[0], x = add[1];
+      const float f[8] = {u.x, u.y, u.z, u.w, x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __fadd_rn(v[i], f[i]);
+    }
+    if (w.allowed != 0xff) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (!(w.allowed >> i & 1)) v[i] = -INFINITY;
+    }
+    uint32_t packed[4];
+    if (!F32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(packed[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
+        v[2 * i] = __uint_as_float(packed[i] << 16);
+        v[2 * i + 1] = __uint_as_float(packed[i] & 0xffff0000u);
+      }
+    }
+    const bool full = i1 >= 0 && i1 + 8 <= P.vocab;
+    if (VEC && full) {
+      if (F32) {
+        *reinterpret_cast<float4*>(o32 + i1) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(o32 + i1 + 4) = make_float4(v[4], v[5], v[6], v[7]);
+      } else {
+        *reinterpret_cast<uint4*>(o16 + i1) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i1 + i < 0 || i1 + i >= P.vocab) {
+          v[i] = __uint_as_float(0x7fc00000u);  // never the largest
+          continue;
+        }
+        if (F32) o32[i1 + i] = v[i];
+        else o16[i1 + i] = (uint16_t)(__float_as_uint(v[i]) >> 16);
+      }
+    }
+    if (P.keys) {
+      const float most = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])),
+                               fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+      if (most > top || (best_z < 0 && most == most)) {
+        top = most;
+        best_z = z;
+      }
+    }
+  };
+
+  for (int z = 0; z < P.spans; ++z) {
+    load(next, z + 1);  // on its way while this span is worked on
+    apply(w, z);
+    w = next;
   }
   if (!P.keys) return;
-  // ---- the greedy key: the thread's largest value, the warp's, and the lowest index that has it
-  float top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = fmaxf(top, i < n ? v[i] : -INFINITY);  // NaN never wins
-  bool any = top != -INFINITY;
-  if (!any) {  // nothing, NaN, or -inf, which is a value too
-#pragma unroll
-    for (int i = 0; i < 8; ++i) any |= i < n && v[i] == v[i];
-  }
-  const uint32_t mine = any ? mc_fkey(top) : 0u;
+  // ---- the greedy key: the warp's largest value; who has it reads its group again for the
+  // lowest token
+  const uint32_t mine = best_z >= 0 ? mc_fkey(top) : 0u;
   const uint32_t most = __reduce_max_sync(0xffffffffu, mine);
   uint32_t at = 0xffffffffu;
-  if (any && mine == most) {
+  if (mine == most && most) {
+    const int i1 = first + best_z * kSpan + tid * 8;
 #pragma unroll
     for (int i = 7; i >= 0; --i)
-      if (i < n && v[i] == top) at = (uint32_t)(i0 + i);
+      if (i1 + i >= 0 && i1 + i < P.vocab &&
+          (F32 ? o32[i1 + i] : mc_bf16_to_f32(o16[i1 + i])) == top)
+        at = (uint32_t)(i1 + i);
   }
   at = __reduce_min_sync(0xffffffffu, at);
   if ((tid & 31) == 0) key_s[tid >> 5] = most ? (unsigned long long)most << 32 | (uint32_t)~at : 0;
@@ -269,8 +339,9 @@ extern "C" int mc_logits_process(mc_ctx* ctx, const void* logits, size_t logits_
   MC_REQUIRE(!allowed || allowed_row || n_allowed >= batch,
              "%s: %d mask rows for a batch of %d (allowed_row is null)", name, n_allowed, batch);
   const size_t size = dtype == MC_DTYPE_F32 ? 4 : 2, far = (size_t)1 << 40;
-  MC_REQUIRE(mc_aligned(logits, size) && mc_aligned(out, size) && mc_aligned(keys, 8),
-             "%s: misaligned rows or keys", name);
+  MC_REQUIRE(mc_aligned(logits, size) && mc_aligned(out, size) && mc_aligned(keys, 8) &&
+                 mc_aligned(counts, 2),
+             "%s: misaligned rows, counts or keys", name);
   MC_REQUIRE(logits_stride <= far && out_stride <= far, "%s: row stride out of range", name);
   MC_REQUIRE(batch <= 1 || out_stride >= (size_t)vocab, "%s: out rows overlap", name);
   const uintptr_t a = (uintptr_t)logits, c = (uintptr_t)out;
@@ -282,17 +353,27 @@ extern "C" int mc_logits_process(mc_ctx* ctx, const void* logits, size_t logits_
   MC_REQUIRE(ctx, "%s: null context", name);
   McDeviceGuard dev(ctx->device);
   MC_CUDA(dev.error());
-  const RulesParams P{logits, logits_stride, vocab, seen, counts, repetition, frequency, presence,
-                      bias_start, bias_ids, bias_vals, n_bias, allowed, allowed_row, n_allowed,
-                      out, out_stride, keys};
-  const bool rows16 = batch == 1 || (logits_stride * size % 16 == 0 && out_stride * size % 16 == 0);
-  const bool vec = mc_aligned(logits, 16) && mc_aligned(out, 16) && rows16 &&
-                   (!counts || (mc_aligned(counts, 16) && (batch == 1 || vocab % 8 == 0)));
-  const dim3 grid((unsigned)(((size_t)vocab + kTokens - 1) / kTokens), (unsigned)batch);
+  RulesParams P{logits, logits_stride, vocab, seen, counts, repetition, frequency, presence,
+                bias_start, bias_ids, bias_vals, n_bias, allowed, allowed_row, n_allowed,
+                out, out_stride, keys, 1};
+  // every row's start the same number of elements behind a 16-byte border (counts: 8 bytes
+  // for float logits, whose groups begin on those)
+  const size_t lane = 16 / size, la = (uintptr_t)logits / size % lane;
+  const bool vec = (uintptr_t)out / size % lane == la &&
+                   (batch == 1 || logits_stride % lane == out_stride % lane) &&
+                   (!counts || ((uintptr_t)counts / 2 % lane == la && mc_aligned(counts, 2) &&
+                                (batch == 1 || (size_t)vocab % lane == logits_stride % lane)));
+  // CTAs a row: as many as one wave leaves it, in runs of at most kSpans spans
+  const int all = (vocab + (vec ? (int)lane - 1 : 0) + kSpan - 1) / kSpan, share = kResident * ctx->num_sms / batch;
+  int spans = share > 0 ? (all + share - 1) / share : kSpans;
+  spans = spans < 1 ? 1 : spans > kSpans ? kSpans : spans;
+  P.spans = spans;
+  const dim3 grid((unsigned)((all + spans - 1) / spans), (unsigned)batch);
   auto fn = dtype == MC_DTYPE_F32
                 ? (vec ? logits_rules_kernel<true, true> : logits_rules_kernel<true, false>)
                 : (vec ? logits_rules_kernel<false, true> : logits_rules_kernel<false, false>);
-  MC_CUDA(mc_launch_pdl(fn, grid, dim3(kThreads), 0, ctx->stream, P));
+  const size_t smem = bias_start ? (size_t)spans * kSpan * sizeof(float) : 0;
+  MC_CUDA(mc_launch_pdl(fn, grid, dim3(kThreads), smem, ctx->stream, P));
   return mc_after_launch("logits_rules_kernel");
 }
 

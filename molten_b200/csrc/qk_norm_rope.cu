@@ -19,8 +19,10 @@
 // that rotate into each other (so no pair crosses threads), for every token of
 // the CTA's batch: its gains, addresses and role stay in registers. A batch's
 // cosines, sines and cache rows are computed once into shared memory by all
-// threads together. Few tokens: a CTA each; many: up to 8 a CTA, 4 tokens'
-// loads in flight a thread.
+// threads together. One wave of CTAs shares the tokens evenly, in batches of
+// up to 8, with the loads of the next 4 in flight (4096 tokens of 32 + 2 x 8
+// heads of 64, 50 MB, mostly in L2: 15 us; 3 CTAs an SM with fewer loads each
+// 15.5 us; a CTA a token, rotation partners by shuffle, 25.6 us).
 #include <cuda_fp8.h>
 #include <math.h>
 
@@ -28,16 +30,17 @@
 
 namespace {
 
-constexpr int kMaxThreads = 512;
+constexpr int kMaxThreads = 384;
 constexpr int kBatch = 8;   // most tokens of a CTA
-constexpr int kFlight = 4;  // tokens whose loads are in flight together
+constexpr int kFlight = 4;    // tokens whose loads are in flight together
+constexpr int kResident = 2;  // CTAs an SM holds at once
 
 struct RopeParams {
   const uint16_t* q;
   const uint16_t* k;
   const uint16_t* v;  // null: V is not written
   size_t q_stride, k_stride, v_stride;
-  int tokens, batch;      // tokens of a CTA: batch (1 to kBatch)
+  int tokens, share, batch;  // tokens of a CTA, and of them at once (1 to kBatch)
   int H, K, rows, group;  // rows = H + K (+ K with v), `group` of them a CTA
   const uint16_t* qw;  // null: no norm
   const uint16_t* kw;
@@ -76,15 +79,22 @@ __device__ __forceinline__ uint32_t pack4_e4m3(const float* f) {
   return lo | hi << 16;
 }
 
+__device__ __forceinline__ void rotate(float& a, float& b, float cosine, float sine) {
+  const float p = a;
+  a = __fmaf_rn(p, cosine, -(b * sine));
+  b = __fmaf_rn(b, cosine, p * sine);
+}
+
 // D: head_dim; F8: e4m3 cache.
 template <int D, bool F8>
-__global__ void __launch_bounds__(kMaxThreads) qk_norm_rope_kernel(const RopeParams P) {
+__global__ void __launch_bounds__(kMaxThreads, kResident) qk_norm_rope_kernel(const RopeParams P) {
   constexpr int L = D / 8;  // threads of a row
-  __shared__ float2 cs[kBatch][D / 2];
+  __shared__ __align__(16) float2 cs[kBatch][D / 2];
   __shared__ uint32_t row_s[kBatch];  // the token's row of head 0 in the cache, all ones: none
   const int tid = threadIdx.x, c = tid % L;
   const int half = P.rot / 2, turned = P.rot / 8;  // threads of a row that rotate
-  const int t0 = blockIdx.x * P.batch, n = min(P.batch, P.tokens - t0);
+  const int t_end = min(P.tokens, (int)(blockIdx.x + 1) * P.share);
+  int t0 = blockIdx.x * P.share;
 
   // ---- this thread's row and its two groups of 4 elements
   const int r = blockIdx.y * P.group + tid / L;
@@ -99,22 +109,28 @@ __global__ void __launch_bounds__(kMaxThreads) qk_norm_rope_kernel(const RopePar
   }
   const uint16_t* src = is_q ? P.q : is_k ? P.k : P.v;
   const size_t stride = is_q ? P.q_stride : is_k ? P.k_stride : P.v_stride;
-  src += (size_t)t0 * stride + (size_t)h * D;
+  src += (size_t)h * D;
   const uint16_t* w = is_q ? P.qw : is_k ? P.kw : nullptr;
+  uint16_t* q_to = P.q_out + (size_t)t0 * P.q_out_stride + (size_t)h * D;
+  void* cache = is_k ? P.kc : P.vc;
+  const uint32_t head_row = (uint32_t)h * P.block_size;
   mc_pdl_launch_dependents();
   mc_pdl_wait();
 
   uint2 xa[kFlight], xb[kFlight];
-  auto load = [&](int t) {
+  auto load = [&](int t) {  // tokens t, t + 1, ...
+    const uint16_t* p = src + (size_t)t * stride;
 #pragma unroll
-    for (int i = 0; i < kFlight; ++i)
-      if (in && t + i < n) {
+    for (int i = 0; i < kFlight; ++i) {
+      if (in && t + i < t_end) {
         // plain loads: q_out may be q
-        xa[i] = *reinterpret_cast<const uint2*>(src + (size_t)(t + i) * stride + 4 * a);
-        xb[i] = *reinterpret_cast<const uint2*>(src + (size_t)(t + i) * stride + 4 * b);
+        xa[i] = *reinterpret_cast<const uint2*>(p + 4 * a);
+        xb[i] = *reinterpret_cast<const uint2*>(p + 4 * b);
       }
+      p += stride;
+    }
   };
-  load(0);
+  load(t0);
   float ga[4], gb[4];
   if (in && w) {
     unpack4(__ldg(reinterpret_cast<const uint2*>(w) + a), ga);
@@ -125,97 +141,95 @@ __global__ void __launch_bounds__(kMaxThreads) qk_norm_rope_kernel(const RopePar
     const float* s = is_k ? P.k_scale : P.v_scale;
     if (s) scale = __fdiv_rn(1.0f, s[h]);
   }
-  for (int i = tid; i < n * half; i += blockDim.x) {
-    const int t = i / half, f = i - t * half;
-    const unsigned long long turn =
-        (unsigned long long)(long long)P.positions[t0 + t] * P.turns[f];
-    // signed fraction of a turn in [-1/2, 1/2), doubled: half turns
-    const float x = __ll2float_rn((long long)turn) * 1.0842021724855044e-19f;  // 2^-63
-    float s, co;
-    sincospif(x, &s, &co);
-    cs[t][f] = make_float2(co, s);
-  }
-  if (tid < n) {
-    const unsigned long long slot = P.slots ? P.slots[t0 + tid] : (unsigned long long)(t0 + tid);
-    uint32_t row = 0xffffffffu;
-    if (slot < P.n_slots) {
-      const uint32_t page = (uint32_t)slot / P.block_size;
-      row = page * P.page_rows + ((uint32_t)slot - page * P.block_size);
-    } else if (slot != MC_KV_SLOT_NONE && P.status && blockIdx.y == 0) {
-      atomicOr(P.status, MC_KV_BAD_SLOT);
+  for (; t0 < t_end; t0 += P.batch) {
+    const int n = min(P.batch, t_end - t0);
+    __syncthreads();  // the batch before is done with the shared arrays
+    for (int i = tid; i < n * half; i += blockDim.x) {
+      const int t = i / half, f = i - t * half;
+      const unsigned long long turn =
+          (unsigned long long)(long long)P.positions[t0 + t] * P.turns[f];
+      // signed fraction of a turn in [-1/2, 1/2), doubled: half turns
+      const float x = __ll2float_rn((long long)turn) * 1.0842021724855044e-19f;  // 2^-63
+      float s, co;
+      sincospif(x, &s, &co);
+      cs[t][f] = make_float2(co, s);
     }
-    row_s[tid] = row;
-  }
-  __syncthreads();
+    if (tid < n) {
+      const unsigned long long slot = P.slots ? P.slots[t0 + tid] : (unsigned long long)(t0 + tid);
+      uint32_t row = 0xffffffffu;
+      if (slot < P.n_slots) {
+        const uint32_t page = (uint32_t)slot / P.block_size;
+        row = page * P.page_rows + ((uint32_t)slot - page * P.block_size);
+      } else if (slot != MC_KV_SLOT_NONE && P.status && blockIdx.y == 0) {
+        atomicOr(P.status, MC_KV_BAD_SLOT);
+      }
+      row_s[tid] = row;
+    }
+    __syncthreads();
 
-  for (int t = 0; t < n; t += kFlight) {
+    for (int t = 0; t < n; t += kFlight) {
 #pragma unroll
-    for (int i = 0; i < kFlight; ++i) {
-      if (t + i >= n) break;  // the same for the whole CTA
-      float x[4], y[4];
-      unpack4(xa[i], x);
-      unpack4(xb[i], y);
-      if (P.qw || P.kw) {
-        float ss = 0.0f;
+      for (int i = 0; i < kFlight; ++i) {
+        if (t + i >= n) break;  // the same for the whole CTA
+        float x[4], y[4];
+        unpack4(xa[i], x);
+        unpack4(xb[i], y);
+        if (P.qw || P.kw) {
+          float ss = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) ss = __fmaf_rn(x[j], x[j], __fmaf_rn(y[j], y[j], ss));
+          for (int j = 0; j < 4; ++j) ss = __fmaf_rn(x[j], x[j], __fmaf_rn(y[j], y[j], ss));
 #pragma unroll
-        for (int m = 1; m < L; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-        if (w) {
-          const float inv = rsqrtf(__fmaf_rn(ss, 1.0f / D, P.eps));
+          for (int m = 1; m < L; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+          if (w) {
+            const float inv = rsqrtf(__fmaf_rn(ss, 1.0f / D, P.eps));
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            x[j] = x[j] * inv * ga[j];
-            y[j] = y[j] * inv * gb[j];
+            for (int j = 0; j < 4; ++j) {
+              x[j] = x[j] * inv * ga[j];
+              y[j] = y[j] * inv * gb[j];
+            }
+          }
+        }
+        if (turns_here) {
+          // this thread's four frequencies: 4 c .. 4 c + 3
+          const float4 e = *reinterpret_cast<const float4*>(&cs[t + i][4 * c]);
+          const float4 f = *reinterpret_cast<const float4*>(&cs[t + i][4 * c + 2]);
+          if (P.interleaved) {
+            rotate(x[0], x[1], e.x, e.y);
+            rotate(x[2], x[3], e.z, e.w);
+            rotate(y[0], y[1], f.x, f.y);
+            rotate(y[2], y[3], f.z, f.w);
+          } else {
+            rotate(x[0], y[0], e.x, e.y);
+            rotate(x[1], y[1], e.z, e.w);
+            rotate(x[2], y[2], f.x, f.y);
+            rotate(x[3], y[3], f.z, f.w);
+          }
+        }
+        if (!in) continue;
+        if (is_q) {
+          *reinterpret_cast<uint2*>(q_to + 4 * a) = pack4(x);
+          *reinterpret_cast<uint2*>(q_to + 4 * b) = pack4(y);
+          q_to += P.q_out_stride;
+        } else if (row_s[t + i] != 0xffffffffu) {
+          const size_t at = (size_t)(row_s[t + i] + head_row) * D;
+          if (F8) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              x[j] *= scale;
+              y[j] *= scale;
+            }
+            uint8_t* to = static_cast<uint8_t*>(cache) + at;
+            *reinterpret_cast<uint32_t*>(to + 4 * a) = pack4_e4m3(x);
+            *reinterpret_cast<uint32_t*>(to + 4 * b) = pack4_e4m3(y);
+          } else {
+            uint16_t* to = static_cast<uint16_t*>(cache) + at;
+            *reinterpret_cast<uint2*>(to + 4 * a) = pack4(x);
+            *reinterpret_cast<uint2*>(to + 4 * b) = pack4(y);
           }
         }
       }
-      if (turns_here) {
-        if (P.interleaved) {
-#pragma unroll
-          for (int j = 0; j < 4; j += 2) {
-            const float2 e = cs[t + i][4 * c + j / 2], f = cs[t + i][4 * c + 2 + j / 2];
-            const float p = x[j], q = y[j];
-            x[j] = __fmaf_rn(p, e.x, -(x[j + 1] * e.y));
-            x[j + 1] = __fmaf_rn(x[j + 1], e.x, p * e.y);
-            y[j] = __fmaf_rn(q, f.x, -(y[j + 1] * f.y));
-            y[j + 1] = __fmaf_rn(y[j + 1], f.x, q * f.y);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 e = cs[t + i][4 * c + j];
-            const float p = x[j];
-            x[j] = __fmaf_rn(p, e.x, -(y[j] * e.y));
-            y[j] = __fmaf_rn(y[j], e.x, p * e.y);
-          }
-        }
-      }
-      if (!in) continue;
-      if (is_q) {
-        uint16_t* to = P.q_out + (size_t)(t0 + t + i) * P.q_out_stride + (size_t)h * D;
-        *reinterpret_cast<uint2*>(to + 4 * a) = pack4(x);
-        *reinterpret_cast<uint2*>(to + 4 * b) = pack4(y);
-      } else if (row_s[t + i] != 0xffffffffu) {
-        const size_t at = ((size_t)row_s[t + i] + (size_t)h * P.block_size) * D;
-        void* cache = is_k ? P.kc : P.vc;
-        if (F8) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            x[j] *= scale;
-            y[j] *= scale;
-          }
-          uint8_t* to = static_cast<uint8_t*>(cache) + at;
-          *reinterpret_cast<uint32_t*>(to + 4 * a) = pack4_e4m3(x);
-          *reinterpret_cast<uint32_t*>(to + 4 * b) = pack4_e4m3(y);
-        } else {
-          uint16_t* to = static_cast<uint16_t*>(cache) + at;
-          *reinterpret_cast<uint2*>(to + 4 * a) = pack4(x);
-          *reinterpret_cast<uint2*>(to + 4 * b) = pack4(y);
-        }
-      }
+      load(t0 + min(t + kFlight, n));
     }
-    load(t + kFlight);
   }
 }
 
@@ -225,10 +239,12 @@ int launch_rope(mc_ctx* ctx, RopeParams& P) {
   const int most = kMaxThreads / (D / 8), parts = (P.rows + most - 1) / most;
   P.group = (P.rows + parts - 1) / parts;
   const int threads = (P.group * (D / 8) + 31) / 32 * 32;
-  // a CTA takes more tokens once every SM has some 4 of them
-  const long long some = 4ll * ctx->num_sms, batch = ((long long)P.tokens * parts + some - 1) / some;
-  P.batch = batch > kBatch ? kBatch : (int)batch;
-  const dim3 grid((unsigned)((P.tokens + P.batch - 1) / P.batch), (unsigned)parts);
+  // one wave: equal shares of the tokens for every CTA that fits, in equal batches
+  const int slots = kResident * ctx->num_sms / parts;
+  P.share = (P.tokens + slots - 1) / slots;
+  const int batches = (P.share + kBatch - 1) / kBatch;
+  P.batch = (P.share + batches - 1) / batches;
+  const dim3 grid((unsigned)((P.tokens + P.share - 1) / P.share), (unsigned)parts);
   MC_CUDA(mc_launch_pdl(qk_norm_rope_kernel<D, F8>, grid, dim3(threads), 0, ctx->stream, P));
   return mc_after_launch("qk_norm_rope_kernel");
 }
@@ -271,7 +287,7 @@ extern "C" int mc_qk_norm_rope(mc_ctx* ctx, const uint16_t* q, size_t q_stride, 
   int rc = mc_check_kv_cache(name, k_cache, v_cache, kv_dtype, num_blocks, block_size,
                              block_stride, n_kv_heads, head_dim, k_scale, v_scale);
   if (rc) return rc;
-  MC_REQUIRE(n_tokens >= 0, "%s: n_tokens %d", name, n_tokens);
+  MC_REQUIRE(n_tokens >= 0 && n_tokens <= (1 << 30), "%s: n_tokens %d out of range", name, n_tokens);
   if (n_tokens == 0) return MC_OK;
   MC_REQUIRE(n_heads >= 1 && n_heads <= 16384, "%s: n_heads %d out of range", name, n_heads);
   MC_REQUIRE(rot_dim >= 0 && rot_dim % 16 == 0 && rot_dim <= head_dim,
@@ -303,7 +319,7 @@ extern "C" int mc_qk_norm_rope(mc_ctx* ctx, const uint16_t* q, size_t q_stride, 
   MC_REQUIRE(ctx, "%s: null context", name);
   McDeviceGuard dev(ctx->device);
   MC_CUDA(dev.error());
-  RopeParams P{q, k, v, q_stride, k_stride, v_stride, n_tokens, 1, n_heads, n_kv_heads,
+  RopeParams P{q, k, v, q_stride, k_stride, v_stride, n_tokens, 1, 1, n_heads, n_kv_heads,
                n_heads + n_kv_heads * (v ? 2 : 1), 0, q_norm_w, k_norm_w, eps, positions,
                reinterpret_cast<const unsigned long long*>(turns), rot_dim, interleaved, q_out,
                q_out_stride, reinterpret_cast<const unsigned long long*>(slots), k_cache, v_cache,
