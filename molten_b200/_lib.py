@@ -183,4 +183,6 @@ def check(rc: int) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(lib(), name)(*args))
+    rc = getattr(_lib or lib(), name)(*args)
+    if rc != MC_OK:
+        check(rc)

@@ -40,7 +40,7 @@ def raise_on_status(status: torch.Tensor, what: str) -> None:
 
 
 def _on(ctx: Context, t: torch.Tensor) -> bool:
-    return t.is_cuda and t.get_device() == (ctx.device.index or 0)
+    return t.get_device() == ctx.index
 
 
 def _ptr(ctx: Context, t: torch.Tensor | None, dtype: torch.dtype, what: str,
@@ -49,8 +49,8 @@ def _ptr(ctx: Context, t: torch.Tensor | None, dtype: torch.dtype, what: str,
     context's device."""
     if t is None:
         return None
-    if t.dtype != dtype or not _on(ctx, t) or not t.is_contiguous() or (
-            numel is not None and t.numel() != numel):
+    if (t.dtype is not dtype or t.get_device() != ctx.index or not t.is_contiguous()
+            or (numel is not None and t.numel() != numel)):
         ensure(t.dtype == dtype, f"{what} expects {dtype}")
         ensure(_on(ctx, t), f"{what} must be on {ctx.device}")
         ensure(t.is_contiguous(), f"{what} must be contiguous")
@@ -58,15 +58,18 @@ def _ptr(ctx: Context, t: torch.Tensor | None, dtype: torch.dtype, what: str,
     return t.data_ptr()
 
 
-def _rows(ctx: Context, t: torch.Tensor, what: str) -> tuple[int, int]:
+def _rows(ctx: Context, t: torch.Tensor, shape: torch.Size, what: str) -> tuple[int, int]:
     """Address and token stride of bf16 rows [tokens, heads, dim] whose heads
     are contiguous (a part of a fused projection row is fine)."""
-    ensure(t.dim() == 3 and t.dtype == torch.bfloat16, f"{what} expects BF16 [rows, heads, dim]")
-    ensure(_on(ctx, t), f"{what} must be on {ctx.device}")
-    s = t.stride()
-    ensure((s[2] == 1 or t.shape[2] == 1) and (s[1] == t.shape[2] or t.shape[1] == 1),
-           f"{what}: a row's heads must be contiguous")
-    return t.data_ptr(), s[0]
+    if t.shape != shape or t.dtype is not torch.bfloat16 or t.get_device() != ctx.index:
+        ensure(t.dtype == torch.bfloat16 and t.dim() == 3, f"{what} expects BF16 [rows, heads, dim]")
+        ensure(_on(ctx, t), f"{what} must be on {ctx.device}")
+        ensure(False, f"{what} shape")
+    token, head, one = t.stride()
+    if one != 1 or head != shape[2]:
+        ensure((one == 1 or shape[2] == 1) and (head == shape[2] or shape[1] == 1),
+               f"{what}: a row's heads must be contiguous")
+    return t.data_ptr(), token
 
 
 @dataclass
@@ -96,6 +99,8 @@ class KvCache:
         dt = _lib.DTYPE_BF16 if k.dtype == torch.bfloat16 else _lib.DTYPE_E4M3
         p = lambda s: None if s is None else s.data_ptr()  # noqa: E731
         stride = k.stride(0) if k.shape[0] > 1 else heads * size * dim
+        self.n_kv_heads, self.head_dim = heads, dim
+        self._index = k.get_device()
         self._where = (k.data_ptr(), v.data_ptr(), dt, k.shape[0], size, stride)
         self._scales = (p(self.k_scale), p(self.v_scale))
 
@@ -178,16 +183,17 @@ def qk_norm_rope(ctx: Context, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
     dim] into the cache at slots [T] (int64, -1: not written; None: slot t),
     with v's rows beside them (None: V is there already). ``turns``: rope_turns
     of the rotated dimensions on the device (None: no rotation)."""
-    T, H, D = q.shape
-    nb, heads, size, dim = cache.k.shape
-    ensure(tuple(k.shape) == (T, heads, D) and dim == D, "qk_norm_rope: k rows match the cache")
-    ensure(q_out.shape == q.shape, "qk_norm_rope: q_out shape")
-    qp, qs = _rows(ctx, q, "q")
-    kp, ks = _rows(ctx, k, "k")
-    vp, vs = (None, 0) if v is None else _rows(ctx, v, "v")
-    ensure(v is None or v.shape == k.shape, "qk_norm_rope: v shape")
-    op, os = _rows(ctx, q_out, "q_out")
-    ensure(_on(ctx, cache.k), f"the cache must be on {ctx.device}")
+    shape = q.shape
+    ensure(len(shape) == 3, "qk_norm_rope: q expects [rows, heads, dim]")
+    T, H, D = shape
+    heads = cache.n_kv_heads
+    ensure(cache.head_dim == D and tuple(k.shape) == (T, heads, D),
+           "qk_norm_rope: k rows match the cache")
+    qp, qs = _rows(ctx, q, shape, "q")
+    kp, ks = _rows(ctx, k, k.shape, "k")
+    vp, vs = (None, 0) if v is None else _rows(ctx, v, k.shape, "v")
+    op, os = _rows(ctx, q_out, shape, "q_out")
+    ensure(cache._index == ctx.index, f"the cache must be on {ctx.device}")
     rot = 0 if turns is None else 2 * turns.numel()
     ensure(rot == 0 or positions is not None, "qk_norm_rope: rotation needs positions")
     b16 = torch.bfloat16
@@ -215,19 +221,19 @@ def paged_attention(ctx: Context, q: torch.Tensor, cache: KvCache, block_table: 
     kv_lens[row] keys of block_table[row_req[row]] (None: row), the last
     ``window`` of them if positive; out like q, lse f32 [rows, heads] optional.
     ``scale``: 1 / sqrt(dim) if None. A row without keys gives zeros and -inf."""
-    rows, H, D = q.shape
-    nb, heads, size, dim = cache.k.shape
-    ensure(dim == D and H % heads == 0, "paged_attention: query heads match the cache")
-    ensure(out.shape == q.shape, "paged_attention: out shape")
+    shape = q.shape
+    ensure(len(shape) == 3, "paged_attention: q expects [rows, heads, dim]")
+    rows, H, D = shape
+    heads = cache.n_kv_heads
+    ensure(cache.head_dim == D and H % heads == 0, "paged_attention: query heads match the cache")
     ensure(block_table.dim() == 2, "block table [requests, width]")
-    ensure(_on(ctx, cache.k), f"the cache must be on {ctx.device}")
-    qp, qs = _rows(ctx, q, "q")
-    op, os = _rows(ctx, out, "out")
+    ensure(cache._index == ctx.index, f"the cache must be on {ctx.device}")
+    qp, qs = _rows(ctx, q, shape, "q")
+    op, os = _rows(ctx, out, shape, "out")
     i32 = torch.int32
-    where = cache._where
-    _lib.call("mc_paged_attention", ctx.handle, qp, qs, rows, H, *where, heads, D, *cache._scales,
-              _ptr(ctx, block_table, i32, "block_table"), block_table.shape[0],
-              block_table.shape[1], _ptr(ctx, kv_lens, i32, "kv_lens", rows),
+    n_req, width = block_table.shape
+    _lib.call("mc_paged_attention", ctx.handle, qp, qs, rows, H, *cache._where, heads, D,
+              *cache._scales, _ptr(ctx, block_table, i32, "block_table"), n_req, width, _ptr(ctx, kv_lens, i32, "kv_lens", rows),
               _ptr(ctx, row_req, i32, "row_req", rows), window,
               1.0 / math.sqrt(D) if scale is None else scale, op, os,
               _ptr(ctx, lse, torch.float32, "lse", rows * H),

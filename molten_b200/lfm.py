@@ -52,6 +52,11 @@ def raise_on_status(word: torch.Tensor, what: str) -> None:
         raise _lib.McError(_lib.MC_ETIMEOUT, f"{what}: status 0x{v:x} ({why})")
 
 
+# The current stream's address without a Stream object around it (2 us less a call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 class Context:
     """MetalContext + ComputePass stand-in: one device and stream (metal.rs:91-400).
 
@@ -62,16 +67,22 @@ class Context:
     def __init__(self, device: int | torch.device = 0, stream: torch.cuda.Stream | None = None):
         dev = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
         self.device = dev
+        self.index = dev.index or 0
         self._fixed_stream = stream
         h = _lib.C.c_void_p()
         s = (stream or torch.cuda.current_stream(dev)).cuda_stream
         _lib.check(_lib.lib().mc_create(dev.index or 0, s, _lib.C.byref(h)))
         self.h = h
+        self._stream = s  # the library's context has this one
 
     @property
     def handle(self):
-        s = (self._fixed_stream or torch.cuda.current_stream(self.device)).cuda_stream
-        _lib.check(_lib.lib().mc_set_stream(self.h, s))
+        if self._fixed_stream is not None:
+            return self.h
+        s = _raw_stream(self.index)
+        if s != self._stream:
+            _lib.check(_lib.lib().mc_set_stream(self.h, s))
+            self._stream = s
         return self.h
 
     def commit_wait(self) -> None:

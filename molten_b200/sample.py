@@ -148,11 +148,12 @@ class LogitsRules:
     allowed_row: torch.Tensor | None = None
 
 
-def _rows2(ctx: Context, t: torch.Tensor, what: str) -> tuple[int, int]:
-    ensure(t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1),
-           f"{what}: rows [batch, vocab], each contiguous")
-    ensure(_on(ctx, t), f"{what} must be on {ctx.device}")
-    return t.data_ptr(), t.stride(0)
+def _vocab_rows(ctx: Context, t: torch.Tensor, what: str) -> tuple[int, int]:
+    row, one = t.stride()
+    if one != 1 or not _on(ctx, t):
+        ensure(one == 1 or t.shape[1] == 1, f"{what}: rows [batch, vocab], each contiguous")
+        ensure(_on(ctx, t), f"{what} must be on {ctx.device}")
+    return t.data_ptr(), row
 
 
 def logits_process(ctx: Context, logits: torch.Tensor, out: torch.Tensor, rules: LogitsRules,
@@ -161,11 +162,12 @@ def logits_process(ctx: Context, logits: torch.Tensor, out: torch.Tensor, rules:
     ``out`` (logits itself, or apart from it): repetition, frequency and
     presence, biases, then the grammar mask. ``best`` (int64 [batch], zero on
     entry): takes the greedy keys that lfm.token_tail reads."""
-    B, V = logits.shape
-    ensure(logits.dtype in (torch.bfloat16, torch.float32) and out.dtype == logits.dtype and
-           out.shape == logits.shape, "logits_process: logits and out, BF16 or F32")
-    lp, ls = _rows2(ctx, logits, "logits")
-    op, os = _rows2(ctx, out, "out")
+    shape, dtype = logits.shape, logits.dtype
+    ensure(len(shape) == 2 and dtype in (torch.bfloat16, torch.float32) and out.dtype is dtype
+           and out.shape == shape, "logits_process: logits and out [batch, vocab], BF16 or F32")
+    B, V = shape
+    lp, ls = _vocab_rows(ctx, logits, "logits")
+    op, os = _vocab_rows(ctx, out, "out")
     W = (V + 31) // 32
     i32, f32 = torch.int32, torch.float32
     r = rules
@@ -173,7 +175,7 @@ def logits_process(ctx: Context, logits: torch.Tensor, out: torch.Tensor, rules:
     ensure(r.allowed is None or (r.allowed.dim() == 2 and r.allowed.shape[1] == W),
            "allowed shape")
     _lib.call("mc_logits_process", ctx.handle, lp, ls,
-              _lib.DTYPE_BF16 if logits.dtype == torch.bfloat16 else _lib.DTYPE_F32, V, B,
+              _lib.DTYPE_BF16 if dtype is torch.bfloat16 else _lib.DTYPE_F32, V, B,
               _ptr(ctx, r.seen, i32, "seen", B * W),
               _ptr(ctx, r.counts, torch.int16, "counts", B * V),
               _ptr(ctx, r.repetition, f32, "repetition", B),

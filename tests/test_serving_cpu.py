@@ -194,7 +194,7 @@ def test_python_checks_come_first():
     from molten_b200 import kv, sample
 
     class Ctx:
-        device = torch.device("cuda", 0)
+        device, index = torch.device("cuda", 0), 0
         handle = property(lambda s: pytest.fail("the call went on"))
 
     ctx = Ctx()
