@@ -12,16 +12,18 @@
 // running sums). A request is admitted whole or not at all.
 //
 // The work is a few hundred bytes to a few hundred KB, bound by latency: one
-// CTA while the token maps fit its threads, else the maps (20 bytes a token)
-// in a second, chained launch. The first launch writes the map entries of
-// each request's first token; their position and kv_len tell the second
-// launch the request's old length and whether it was admitted, so
+// CTA (of as who threads as there are requests or rows to map where that
+// bounds the pages too, else the most), with what the maps need in shared
+// memory; above kMapsInPlan rows the maps (20 bytes a
+// token) go to a second, chained launch. The first launch writes the map
+// entries of each request's first token; their position and kv_len tell the
+// second launch the request's old length and whether it was admitted, so
 // `seq_lens` may be `lens` itself.
 #include "kv_common.cuh"
 
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 1024;  // most threads; requests of a chunk
 constexpr int kWarpsP = kThreads / 32;
 
 struct PlanParams {
@@ -56,17 +58,18 @@ __device__ __forceinline__ long long block_scan(long long v, long long* warp_sum
   if (lane == 31) warp_sums[warp] = v;
   __syncthreads();
   if (warp == 0) {
-    long long w = lane < kWarpsP ? warp_sums[lane] : 0;
+    const int warps = blockDim.x >> 5;
+    long long w = lane < warps ? warp_sums[lane] : 0;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
+    for (int d = 1; d < kWarpsP; d <<= 1) {
       const long long o = __shfl_up_sync(0xffffffffu, w, d);
       if (lane >= d) w += o;
     }
-    if (lane < kWarpsP) warp_sums[lane] = w;
+    if (lane < warps) warp_sums[lane] = w;
   }
   __syncthreads();
   if (warp > 0) v += warp_sums[warp - 1];
-  total = warp_sums[kWarpsP - 1];
+  total = warp_sums[(blockDim.x >> 5) - 1];
   __syncthreads();
   return v;
 }
@@ -81,6 +84,45 @@ __device__ __forceinline__ int upper_bound(const T* a, int n, T x) {
     else hi = mid;
   }
   return lo;
+}
+
+// Shares out the pages of a chunk's requests: fn(i, j, n) for page j of the n
+// pages of request i, this thread's being request threadIdx.x with n pages.
+// One or two are done by the request's own thread, up to kWarpPages by one warp
+// together, more by the whole block. Every thread of the block calls it.
+constexpr int kWarpPages = 1024;
+template <typename F>
+__device__ __forceinline__ void share_pages(int n, int* lists, int* count_s, F&& fn) {
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, threads = blockDim.x;
+  // who they are and how many pages: for a warp from the front, for the block from the back
+  int* who = lists;
+  int* pages_of = lists + threads;
+  if (t < 2) count_s[t] = 0;
+  __syncthreads();
+  int at = -1;
+  if (n > kWarpPages) at = threads - 1 - atomicAdd(count_s + 1, 1);
+  else if (n > 2) at = atomicAdd(count_s, 1);
+  if (at >= 0) {
+    who[at] = t;
+    pages_of[at] = n;
+  }
+  if (n == 1 || n == 2) {
+    fn(t, 0, n);
+    if (n == 2) fn(t, 1, n);
+  }
+  __syncthreads();
+  const int n_warp = count_s[0], n_block = count_s[1];
+  for (int k = warp; k < n_warp; k += threads >> 5) {
+    const int i = who[k], pages = pages_of[k];
+#pragma unroll 4
+    for (int j = lane; j < pages; j += 32) fn(i, j, pages);
+  }
+  for (int k = 0; k < n_block; ++k) {
+    const int i = who[threads - 1 - k], pages = pages_of[threads - 1 - k];
+#pragma unroll 4
+    for (int j = t; j < pages; j += threads) fn(i, j, pages);
+  }
+  __syncthreads();
 }
 
 // The maps of token row t (row_start and the first rows' entries written).
@@ -111,25 +153,27 @@ __device__ __forceinline__ void map_token(const PlanParams& P, int t) {
   P.slots[t] = slot;
 }
 
+// MAPS: at most kThreads requests and kMapsInPlan rows, whose maps are written too.
 template <bool MAPS>
 __global__ void __launch_bounds__(kThreads) plan_kernel(const PlanParams P) {
-  mc_pdl_launch_dependents();
-  mc_pdl_wait();
   __shared__ long long warp_sums[kWarpsP];
   __shared__ long long taken_s[kThreads];  // inclusive fresh-page sums of the chunk
   __shared__ int have_s[kThreads];         // pages held; -1: not admitted
+  __shared__ int start_s[MAPS ? kThreads + 1 : 1], len_s[MAPS ? kThreads : 1];
+  __shared__ int lists_s[2 * kThreads], count_s[2];
   __shared__ unsigned long long used_s;
   __shared__ uint32_t status_s;
-  const int t = threadIdx.x;
+  const int t = threadIdx.x, threads = blockDim.x;
   if (t == 0) {
     used_s = 0;
     status_s = 0;
-    P.row_start[0] = 0;
   }
+  mc_pdl_launch_dependents();
+  mc_pdl_wait();
   const long long bs = P.block_size;
   const int nf = min(max(*P.n_free, 0), P.free_len);
   long long rows = 0, pages = 0;  // sums of the chunks before
-  for (int r0 = 0; r0 < P.n_req; r0 += kThreads) {
+  for (int r0 = 0; r0 < P.n_req; r0 += threads) {
     const int r = r0 + t;
     const bool in = r < P.n_req;
     long long len = in ? P.lens[r] : 0, add = in ? (P.new_lens ? P.new_lens[r] : 1) : 0;
@@ -160,26 +204,28 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const PlanParams P) {
     }
     taken_s[t] = taken;
     have_s[t] = ok ? (int)have : -1;
+    const int end32 = (int)min(row_end, (long long)INT32_MAX);
+    if (MAPS) {
+      start_s[t + 1] = end32;
+      len_s[t] = (int)len;
+    }
     if (in) {
       if (ok && need > 0) atomicMax(&used_s, (unsigned long long)(pages + taken));
       if (st) atomicOr(&status_s, st);
       const long long first = row_end - add;
-      P.row_start[r + 1] = (int)min(row_end, (long long)INT32_MAX);
+      if (r == 0) P.row_start[0] = 0;
+      P.row_start[r + 1] = end32;
       P.seq_lens[r] = (int)(ok ? len + add : len);
-      if (add > 0 && first < P.max_tokens) {
+      if (!MAPS && add > 0 && first < P.max_tokens) {
         P.positions[first] = (int)len;
         P.kv_lens[first] = ok ? (int)len + 1 : 0;
       }
     }
     __syncthreads();
-    const int n = min(P.n_req - r0, kThreads);
-    for (long long e = t; e < total; e += kThreads) {
-      const int i = upper_bound(taken_s, n, e);
-      const int h = have_s[i];
-      if (h < 0) continue;
-      const long long before = i ? taken_s[i - 1] : 0;
-      P.table[(size_t)(r0 + i) * P.width + h + (e - before)] = P.free_list[nf - 1 - (pages + e)];
-    }
+    share_pages(ok ? (int)need : 0, lists_s, count_s, [&](int i, int j, int n) {
+      const long long e = pages + taken_s[i] - n + j;
+      P.table[(size_t)(r0 + i) * P.width + have_s[i] + j] = __ldg(P.free_list + (nf - 1 - e));
+    });
     pages += total;
     __syncthreads();
   }
@@ -187,9 +233,25 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const PlanParams P) {
     *P.n_free_out = nf - (int)used_s;
     if (P.status && status_s) atomicOr(P.status, status_s);
   }
-  if (MAPS) {
-    __syncthreads();
-    for (int i = t; i < P.max_tokens; i += kThreads) map_token(P, i);
+  if (!MAPS) return;
+  // the table entries written above are seen behind the barrier
+  for (int i = t; i < P.max_tokens; i += threads) {
+    int pos = 0, req = -1, kv_len = 0;
+    unsigned long long slot = MC_KV_SLOT_NONE;
+    if (i < rows) {
+      req = upper_bound(start_s + 1, P.n_req, i);
+      const long long at = (long long)len_s[req] + i - (req ? start_s[req] : 0);
+      pos = (int)min(at, (long long)INT32_MAX);
+      if (have_s[req] >= 0) {
+        kv_len = pos + 1;
+        const int page = P.table[(size_t)req * P.width + pos / P.block_size];
+        if (page >= 0) slot = (unsigned long long)page * P.block_size + pos % P.block_size;
+      }
+    }
+    P.positions[i] = pos;
+    P.token_req[i] = req;
+    P.kv_lens[i] = kv_len;
+    P.slots[i] = slot;
   }
 }
 
@@ -219,11 +281,12 @@ __global__ void __launch_bounds__(kThreads) release_kernel(const ReleaseParams P
   mc_pdl_wait();
   __shared__ long long warp_sums[kWarpsP];
   __shared__ long long given_s[kThreads];
+  __shared__ int lists_s[2 * kThreads], count_s[2];
   const int t = threadIdx.x;
+  const int threads = blockDim.x;
   const long long nf = min(max(*P.n_free, 0), P.free_len);
-  __syncthreads();
   long long pages = 0;
-  for (int r0 = 0; r0 < P.n_req; r0 += kThreads) {
+  for (int r0 = 0; r0 < P.n_req; r0 += threads) {
     const int r = r0 + t;
     long long held = 0;
     if (r < P.n_req) {
@@ -236,13 +299,10 @@ __global__ void __launch_bounds__(kThreads) release_kernel(const ReleaseParams P
     long long total;
     given_s[t] = block_scan(held, warp_sums, total);
     __syncthreads();
-    const int n = min(P.n_req - r0, kThreads);
-    for (long long e = t; e < total; e += kThreads) {
-      const int i = upper_bound(given_s, n, e);
-      const long long j = e - (i ? given_s[i - 1] : 0);
-      const long long at = nf + pages + e;
-      if (at < P.free_len) P.free_list[at] = P.table[(size_t)(r0 + i) * P.width + j];
-    }
+    share_pages((int)held, lists_s, count_s, [&](int i, int j, int n) {
+      const long long at = nf + pages + given_s[i] - n + j;
+      if (at < P.free_len) P.free_list[at] = __ldg(P.table + (size_t)(r0 + i) * P.width + j);
+    });
     pages += total;
     __syncthreads();
   }
@@ -253,8 +313,14 @@ __global__ void __launch_bounds__(kThreads) release_kernel(const ReleaseParams P
   }
 }
 
-// Above this many token rows the maps go to a launch of their own.
+// Above this who token rows the maps go to a launch of their own.
 constexpr int kMapsInPlan = 2048;
+
+// A thread for each request and row, whole warps.
+int plan_threads(int n_req, int rows) {
+  const int n = n_req > rows ? n_req : rows;
+  return n >= kThreads ? kThreads : (n + 31) / 32 * 32;
+}
 
 }  // namespace
 
@@ -280,8 +346,9 @@ extern "C" int mc_kv_plan(mc_ctx* ctx, const int32_t* lens, const int32_t* new_l
   const PlanParams P{lens, new_lens, n_req, block_size, block_table, table_width, free_list,
                      n_free, free_len, seq_lens, n_free_out, row_start, positions, token_req,
                      kv_lens, reinterpret_cast<unsigned long long*>(slots), max_tokens, status};
-  if (max_tokens <= kMapsInPlan) {
-    MC_CUDA(mc_launch_pdl(plan_kernel<true>, dim3(1), dim3(kThreads), 0, ctx->stream, P));
+  if (max_tokens <= kMapsInPlan && n_req <= kThreads) {
+    MC_CUDA(mc_launch_pdl(plan_kernel<true>, dim3(1), dim3(plan_threads(n_req, max_tokens)), 0,
+                          ctx->stream, P));
     return mc_after_launch("plan_kernel");
   }
   MC_CUDA(mc_launch_pdl(plan_kernel<false>, dim3(1), dim3(kThreads), 0, ctx->stream, P));
