@@ -46,11 +46,19 @@ inline void check(int rc) {
   }
 }
 
-// DType (tensor.rs); U64 holds the argmax keys of the head.
-enum class DType { BF16, F32, U32, U64 };
+// DType (tensor.rs); U64 holds the argmax keys of the head and the cache slots,
+// U32 also the int32 arrays of the paged cache; E4M3 and U16 are the 8-bit cache
+// and the token counts.
+enum class DType { BF16, F32, U32, U64, E4M3, U16 };
 
 inline size_t dtype_size(DType d) {
-  return d == DType::BF16 ? 2 : (d == DType::U64 ? 8 : 4);
+  switch (d) {
+    case DType::E4M3: return 1;
+    case DType::BF16:
+    case DType::U16: return 2;
+    case DType::U64: return 8;
+    default: return 4;
+  }
 }
 
 // A device buffer view: pointer (buffer + offset), shape, dtype.
@@ -501,6 +509,204 @@ inline void sample_mark(Context& ctx, const Tensor& tok, const Tensor& seen, int
   ensure(tok.numel() == 1 && tok.dtype == DType::U32, "sampled token slot");
   check(mc_sample_mark(ctx.handle(), tok.as<const uint32_t>(), seen.as<uint32_t>(), vocab,
                        nullptr));
+}
+
+// The paged key-value cache: K and V pages [num_blocks][KV heads][block
+// size][head dim] (BF16 or E4M3), pages block_stride elements apart (0: one
+// behind the other), optional F32 scales [KV heads] of an E4M3 cache.
+struct KvCache {
+  Tensor k, v;
+  size_t block_stride = 0;
+  const Tensor* k_scale = nullptr;
+  const Tensor* v_scale = nullptr;
+
+  int num_blocks() const { return (int)k.dim(0); }
+  int n_kv_heads() const { return (int)k.dim(1); }
+  int block_size() const { return (int)k.dim(2); }
+  int head_dim() const { return (int)k.dim(3); }
+  int abi_dtype() const { return k.dtype == DType::E4M3 ? MC_DTYPE_E4M3 : MC_DTYPE_BF16; }
+  size_t stride() const {
+    return block_stride ? block_stride : (size_t)(k.dim(1) * k.dim(2) * k.dim(3));
+  }
+  void check() const {
+    ensure(k.shape.size() == 4 && v.shape == k.shape && v.dtype == k.dtype &&
+               (k.dtype == DType::BF16 || k.dtype == DType::E4M3),
+           "KV cache: k and v are alike, BF16 or E4M3 [blocks][KV heads][block size][head dim]");
+    for (const Tensor* s : {k_scale, v_scale})
+      ensure(!s || (s->dtype == DType::F32 && s->numel() == k.dim(1)), "KV cache scales");
+  }
+};
+
+inline const Tensor& i32(const Tensor& t, int64_t n, const char* what) {
+  ensure(t.dtype == DType::U32 && t.numel() == n, std::string(what) + " shape");
+  return t;
+}
+template <typename T>
+inline T* maybe(const Tensor* t) {
+  return t ? t->as<T>() : nullptr;
+}
+
+// One step's bookkeeping of the paged cache (mc_kv_plan): block_table
+// [requests][width], slots U64 and the token maps [max tokens], row_start
+// [requests + 1]; new_lens and status optional.
+inline void kv_plan(Context& ctx, const Tensor& lens, const Tensor* new_lens, int block_size,
+                    const Tensor& block_table, const Tensor& free_list, const Tensor& n_free,
+                    const Tensor& seq_lens, const Tensor& n_free_out, const Tensor& row_start,
+                    const Tensor& positions, const Tensor& token_req, const Tensor& kv_lens,
+                    const Tensor& slots, const Tensor* status = nullptr) {
+  const int64_t n = lens.numel(), rows = slots.numel();
+  ensure(block_table.shape.size() == 2 && block_table.dim(0) == n && slots.dtype == DType::U64,
+         "kv_plan table and slots");
+  if (new_lens) i32(*new_lens, n, "new_lens");
+  check(mc_kv_plan(ctx.handle(), i32(lens, n, "lens").as<const int32_t>(),
+                   maybe<const int32_t>(new_lens), (int)n, block_size,
+                   i32(block_table, block_table.numel(), "block_table").as<int32_t>(),
+                   (int)block_table.dim(1),
+                   i32(free_list, free_list.numel(), "free_list").as<const int32_t>(),
+                   i32(n_free, 1, "n_free").as<const int32_t>(), (int)free_list.numel(),
+                   i32(seq_lens, n, "seq_lens").as<int32_t>(),
+                   i32(n_free_out, 1, "n_free_out").as<int32_t>(),
+                   i32(row_start, n + 1, "row_start").as<int32_t>(),
+                   i32(positions, rows, "positions").as<int32_t>(),
+                   i32(token_req, rows, "token_req").as<int32_t>(),
+                   i32(kv_lens, rows, "kv_lens").as<int32_t>(), slots.as<uint64_t>(), (int)rows,
+                   maybe<uint32_t>(status)));
+}
+
+// Gives the pages of finished requests back (mc_kv_release).
+inline void kv_release(Context& ctx, const Tensor& done, const Tensor& lens, int block_size,
+                       const Tensor& block_table, const Tensor& free_list, const Tensor& n_free,
+                       const Tensor& lens_out, const Tensor& n_free_out,
+                       const Tensor* status = nullptr) {
+  const int64_t n = lens.numel();
+  ensure(block_table.shape.size() == 2 && block_table.dim(0) == n, "kv_release table");
+  check(mc_kv_release(ctx.handle(), i32(done, n, "done").as<const uint32_t>(),
+                      i32(lens, n, "lens").as<const int32_t>(), (int)n, block_size,
+                      i32(block_table, block_table.numel(), "block_table").as<const int32_t>(),
+                      (int)block_table.dim(1),
+                      i32(free_list, free_list.numel(), "free_list").as<int32_t>(),
+                      i32(n_free, 1, "n_free").as<const int32_t>(), (int)free_list.numel(),
+                      i32(lens_out, n, "lens_out").as<int32_t>(),
+                      i32(n_free_out, 1, "n_free_out").as<int32_t>(), maybe<uint32_t>(status)));
+}
+
+// Norm, rotation and cache write of a step's rows (mc_qk_norm_rope): q, k, v
+// and q_out [tokens][heads][head dim] with element strides between tokens
+// (0: contiguous); v, the gains, positions, turns (U64), slots optional.
+inline void qk_norm_rope(Context& ctx, const Tensor& q, size_t q_stride, const Tensor& k,
+                         size_t k_stride, const Tensor* v, size_t v_stride,
+                         const Tensor* q_norm_w, const Tensor* k_norm_w, float eps,
+                         const Tensor* positions, const Tensor* turns, bool interleaved,
+                         const Tensor& q_out, size_t q_out_stride, const KvCache& cache,
+                         const Tensor* slots, const Tensor* status = nullptr) {
+  cache.check();
+  ensure(q.shape.size() == 3 && q.dtype == DType::BF16 && q_out.shape == q.shape &&
+             q_out.dtype == DType::BF16,
+         "qk_norm_rope q rows");
+  const int64_t T = q.dim(0), D = q.dim(2), K = cache.n_kv_heads();
+  ensure(D == cache.head_dim() && k.shape == std::vector<int64_t>{T, K, D} &&
+             k.dtype == DType::BF16 && (!v || (v->shape == k.shape && v->dtype == DType::BF16)),
+         "qk_norm_rope k rows match the cache");
+  ensure((!q_norm_w || q_norm_w->numel() == D) && (!k_norm_w || k_norm_w->numel() == D),
+         "qk_norm_rope gains");
+  ensure(!turns || (turns->dtype == DType::U64 && positions), "qk_norm_rope turns");
+  if (positions) i32(*positions, T, "positions");
+  ensure(!slots || (slots->dtype == DType::U64 && slots->numel() == T), "qk_norm_rope slots");
+  const size_t qn = (size_t)(q.dim(1) * D), kn = (size_t)(K * D);
+  check(mc_qk_norm_rope(
+      ctx.handle(), q.as<const uint16_t>(), q_stride ? q_stride : qn, k.as<const uint16_t>(),
+      k_stride ? k_stride : kn, maybe<const uint16_t>(v), v_stride ? v_stride : kn, (int)T,
+      (int)q.dim(1), (int)K, (int)D, maybe<const uint16_t>(q_norm_w),
+      maybe<const uint16_t>(k_norm_w), eps, maybe<const int32_t>(positions),
+      maybe<const uint64_t>(turns), turns ? (int)(2 * turns->numel()) : 0, interleaved ? 1 : 0,
+      q_out.as<uint16_t>(), q_out_stride ? q_out_stride : qn, maybe<const uint64_t>(slots),
+      cache.k.data, cache.v.data, cache.abi_dtype(), cache.num_blocks(), cache.block_size(),
+      cache.stride(), maybe<const float>(cache.k_scale), maybe<const float>(cache.v_scale),
+      maybe<uint32_t>(status)));
+}
+
+// Attention of query rows over the paged cache (mc_paged_attention): q and out
+// [rows][heads][head dim] contiguous; row_req, lse, status optional; the
+// workspace (mc_paged_attention_workspace_bytes) zeroed once by the caller.
+inline void paged_attention(Context& ctx, const Tensor& q, const KvCache& cache,
+                            const Tensor& block_table, const Tensor& kv_lens,
+                            const Tensor* row_req, int window, float scale, const Tensor& out,
+                            const Tensor* lse, const Tensor& workspace,
+                            const Tensor* status = nullptr) {
+  cache.check();
+  ensure(q.shape.size() == 3 && q.dtype == DType::BF16 && out.shape == q.shape &&
+             out.dtype == DType::BF16,
+         "paged_attention rows");
+  const int64_t rows = q.dim(0), H = q.dim(1), D = q.dim(2);
+  ensure(D == cache.head_dim() && H % cache.n_kv_heads() == 0,
+         "paged_attention query heads match the cache");
+  ensure(block_table.shape.size() == 2 && block_table.dtype == DType::U32, "paged_attention table");
+  if (row_req) i32(*row_req, rows, "row_req");
+  ensure(!lse || (lse->dtype == DType::F32 && lse->numel() == rows * H), "paged_attention lse");
+  check(mc_paged_attention(
+      ctx.handle(), q.as<const uint16_t>(), (size_t)(H * D), (int)rows, (int)H, cache.k.data,
+      cache.v.data, cache.abi_dtype(), cache.num_blocks(), cache.block_size(), cache.stride(),
+      cache.n_kv_heads(), (int)D, maybe<const float>(cache.k_scale),
+      maybe<const float>(cache.v_scale), block_table.as<const int32_t>(), (int)block_table.dim(0),
+      (int)block_table.dim(1), i32(kv_lens, rows, "kv_lens").as<const int32_t>(),
+      maybe<const int32_t>(row_req), window, scale, out.as<uint16_t>(), (size_t)(H * D),
+      maybe<float>(lse), workspace.data, workspace.nbytes(), maybe<uint32_t>(status)));
+}
+
+// The rules on logits (mc_logits_process); null members leave a rule out.
+struct LogitsRules {
+  const Tensor* seen = nullptr;        // U32 [batch][ceil(vocab / 32)]
+  const Tensor* counts = nullptr;      // U16 [batch][vocab]
+  const Tensor* repetition = nullptr;  // F32 [batch], as the next two
+  const Tensor* frequency = nullptr;
+  const Tensor* presence = nullptr;
+  const Tensor* bias_start = nullptr;  // U32 [batch + 1]
+  const Tensor* bias_ids = nullptr;    // U32, ascending within a row
+  const Tensor* bias_values = nullptr;
+  const Tensor* allowed = nullptr;     // U32 [masks][ceil(vocab / 32)]
+  const Tensor* allowed_row = nullptr; // U32 [batch]
+};
+
+inline void logits_process(Context& ctx, const Tensor& logits, const Tensor& out,
+                           const LogitsRules& r, const Tensor* best = nullptr) {
+  ensure(logits.shape.size() == 2 && out.shape == logits.shape && out.dtype == logits.dtype &&
+             (logits.dtype == DType::BF16 || logits.dtype == DType::F32),
+         "logits_process: logits and out [batch][vocab], BF16 or F32");
+  const int64_t B = logits.dim(0), V = logits.dim(1), W = (V + 31) / 32;
+  auto sized = [&](const Tensor* t, DType d, int64_t n, const char* what) {
+    ensure(!t || (t->dtype == d && t->numel() == n), std::string(what) + " shape");
+  };
+  sized(r.seen, DType::U32, B * W, "seen");
+  sized(r.counts, DType::U16, B * V, "counts");
+  sized(r.repetition, DType::F32, B, "repetition");
+  sized(r.frequency, DType::F32, B, "frequency");
+  sized(r.presence, DType::F32, B, "presence");
+  sized(r.bias_start, DType::U32, B + 1, "bias_start");
+  const int64_t n_bias = r.bias_ids ? r.bias_ids->numel() : 0;
+  sized(r.bias_ids, DType::U32, n_bias, "bias_ids");
+  sized(r.bias_values, DType::F32, n_bias, "bias_values");
+  ensure(!r.allowed || (r.allowed->dtype == DType::U32 && r.allowed->shape.size() == 2 &&
+                        r.allowed->dim(1) == W),
+         "allowed shape");
+  sized(r.allowed_row, DType::U32, B, "allowed_row");
+  sized(best, DType::U64, B, "best");
+  check(mc_logits_process(
+      ctx.handle(), logits.data, (size_t)V,
+      logits.dtype == DType::F32 ? MC_DTYPE_F32 : MC_DTYPE_BF16, (int)V, (int)B,
+      maybe<const uint32_t>(r.seen), maybe<const uint16_t>(r.counts),
+      maybe<const float>(r.repetition), maybe<const float>(r.frequency),
+      maybe<const float>(r.presence), maybe<const int32_t>(r.bias_start),
+      maybe<const uint32_t>(r.bias_ids), maybe<const float>(r.bias_values), (int)n_bias,
+      maybe<const uint32_t>(r.allowed), maybe<const int32_t>(r.allowed_row),
+      r.allowed ? (int)r.allowed->dim(0) : 0, out.data, (size_t)V,
+      maybe<unsigned long long>(best)));
+}
+
+// Counts the drawn tokens in the rules' seen bitmap and counts.
+inline void logits_mark(Context& ctx, const Tensor& tokens, const LogitsRules& r, int vocab) {
+  ensure(tokens.dtype == DType::U32, "drawn tokens");
+  check(mc_logits_mark(ctx.handle(), tokens.as<const uint32_t>(), (int)tokens.numel(),
+                       maybe<uint32_t>(r.seen), maybe<uint16_t>(r.counts), vocab));
 }
 
 // Tensor::write_bytes / contents (tensor.rs:127-146, 165-200): stream-ordered

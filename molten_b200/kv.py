@@ -239,3 +239,48 @@ def paged_attention(ctx: Context, q: torch.Tensor, cache: KvCache, block_table: 
               _ptr(ctx, lse, torch.float32, "lse", rows * H),
               _ptr(ctx, workspace, torch.uint8, "workspace"), workspace.numel(),
               _ptr(ctx, status, i32, "status", 1))
+
+
+class PagedBatch:
+    """The bookkeeping of one batch of requests over paged caches: lengths, block
+    tables and the free list on the device, and the token maps of a step.
+    Every layer's ``KvCache`` has ``num_blocks`` pages of ``block_size``; a
+    request's pages have the same numbers in each of them. ``max_tokens``: token
+    rows of a step (one for each request by default)."""
+
+    def __init__(self, ctx: Context, n_req: int, num_blocks: int, block_size: int,
+                 table_width: int, max_tokens: int | None = None):
+        dev = ctx.device
+        i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device=dev)  # noqa: E731
+        T = n_req if max_tokens is None else max_tokens
+        self.ctx, self.block_size = ctx, block_size
+        self.lens, self.n_free = i32(n_req), i32(1)
+        self.block_table = torch.full((n_req, table_width), -1, dtype=torch.int32, device=dev)
+        self.free_list = torch.arange(num_blocks - 1, -1, -1, dtype=torch.int32, device=dev)
+        self.row_start, self.status = i32(n_req + 1), i32(1)
+        self.positions, self.token_req, self.kv_lens = i32(T), i32(T), i32(T)
+        self.slots = torch.zeros(T, dtype=torch.int64, device=dev)
+        self.clear()
+
+    def clear(self) -> None:
+        """Every request empty, every page free."""
+        self.lens.zero_()
+        self.status.zero_()
+        self.n_free.fill_(self.free_list.numel())
+        self.free_list.copy_(torch.arange(self.free_list.numel() - 1, -1, -1, dtype=torch.int32))
+
+    def plan(self, new_lens: torch.Tensor | None = None) -> None:
+        """The next step: new_lens tokens (None: one each) for the requests."""
+        kv_plan(self.ctx, self.lens, new_lens, self.block_size, self.block_table, self.free_list,
+                self.n_free, self.lens, self.n_free, self.row_start, self.positions,
+                self.token_req, self.kv_lens, self.slots, self.status)
+
+    def release(self, done: torch.Tensor) -> None:
+        """Frees the pages of the requests with done[r] != 0 and empties them."""
+        kv_release(self.ctx, done, self.lens, self.block_size, self.block_table, self.free_list,
+                   self.n_free, self.lens, self.n_free, self.status)
+
+    def check(self) -> None:
+        """Waits for the stream and raises McError if a request was refused or
+        an index was out of range since the last clear()."""
+        raise_on_status(self.status, "paged batch")

@@ -33,6 +33,17 @@ residual stream. The expert part runs one of three ways (``moe_path``):
 The token feeds back on the device, so a step can be captured once in a CUDA
 graph and replayed.
 
+A layer with an ``attn`` entry (a dict: norm_w [2048], qkv the Q4 projection of
+the (heads + 2 KV heads) x head_dim rows, q_norm and k_norm [head_dim], cache a
+``kv.KvCache``) mixes tokens before its projection: p = proj_l(attention(x)),
+with RMSNorm, qkv GEMV, qk_norm_rope and paged_attention over that cache. The
+batch's pages are kept by ``kv`` (a ``kv.PagedBatch``), planned once a step for
+all layers; every row of the batch adds its token to its own request.
+
+``rules`` (a ``sample.LogitsRules``): the requests' penalties, biases and grammar
+masks, applied to the head's logits before the greedy token or the draw; the
+tokens then count towards the penalties.
+
 With ``sampling`` (batch 1, the reference's temperature > 0 path,
 lfm/sample.rs), the head stores its bf16 logits (gemv_quant) and the draw
 (mc_sample_draw) folds the sampled token into the same key the greedy head
@@ -44,13 +55,16 @@ from __future__ import annotations
 
 import torch
 
+from molten_b200 import kv as paged
 from molten_b200 import lfm
+from molten_b200.sample import logits_mark, logits_process
 
 
 class DecodeStack:
     def __init__(self, ctx: lfm.Context, layers: list[dict], head, embed: torch.Tensor,
                  batch: int, n_experts: int = 64, moe_path: str | None = None, sampling=None,
-                 fuse_proj: bool = True):
+                 fuse_proj: bool = True, kv: paged.PagedBatch | None = None, rules=None,
+                 rope_theta: float = 1e6):
         self.ctx, self.layers, self.head, self.embed = ctx, layers, head, embed
         self.sampling = sampling
         lfm.ensure(sampling is None or batch == 1, "sampling decodes one sequence")
@@ -87,11 +101,34 @@ class DecodeStack:
         if self.path == "grouped":
             nb = lfm.moe_prefill_workspace_size(batch, n_experts, H, I)
             self.pws = torch.zeros(nb, dtype=torch.uint8, device=dev)
+        self.kv, self.rules = kv, rules
+        self.attn = None
+        with_attn = [L["attn"] for L in layers if "attn" in L]
+        lfm.ensure(not with_attn or kv is not None, "attention layers need a PagedBatch")
+        if with_attn:
+            lfm.ensure(kv.lens.numel() == batch and kv.slots.numel() == batch,
+                       "the PagedBatch has one token row for each row of the batch")
+            c = with_attn[0]["cache"]
+            D, K = c.head_dim, c.n_kv_heads
+            heads = with_attn[0]["qkv"].out_features // D - 2 * K
+            for A in with_attn:
+                lfm.ensure(A["cache"].head_dim == D and A["cache"].n_kv_heads == K and
+                           A["qkv"].out_features == (heads + 2 * K) * D and heads * D == H and
+                           A["cache"].block_size == kv.block_size, "attention layer shapes")
+            rows = bf(batch, (heads + 2 * K) * D)
+            part = lambda a, n: rows[:, a * D:(a + n) * D].view(batch, n, D)  # noqa: E731
+            self.attn = dict(normed=bf(batch, H), rows=rows, q=part(0, heads), k=part(heads, K),
+                             v=part(heads + K, K), q_out=bf(batch, heads, D),
+                             out=bf(batch, heads, D),
+                             turns=paged.rope_turns(D, rope_theta).to(dev),
+                             ws=paged.paged_attention_workspace(D, dev))
+        self.head_logits = None
+        if sampling is not None or rules is not None:
+            self.head_logits = bf(batch, head.out_features)
         self.sample = None
         if sampling is not None:
             from molten_b200.sample import SampleScratch
             self.sample = SampleScratch(ctx, head.out_features)
-            self.head_logits = bf(head.out_features)
             self.pos = torch.zeros(1, dtype=torch.int32, device=dev)
 
     def start(self, tokens: torch.Tensor, pos: int = 0, seen=()) -> None:
@@ -103,11 +140,25 @@ class DecodeStack:
             self.pos.fill_(pos)
             self.sample.upload_seen(list(seen) + [int(t) for t in tokens.cpu()])
 
+    def _attend(self, A: dict, cur: torch.Tensor) -> torch.Tensor:
+        """The attention of one layer on the rows ``cur``: [B, 2048]."""
+        ctx, b, batch = self.ctx, self.attn, self.kv
+        lfm.add_rmsnorm(ctx, cur, None, A["norm_w"], None, b["normed"])
+        lfm.gemv_quant(ctx, A["qkv"], b["normed"], b["rows"])
+        paged.qk_norm_rope(ctx, b["q"], b["k"], b["v"], A["q_norm"], A["k_norm"], batch.positions,
+                           b["turns"], b["q_out"], A["cache"], batch.slots, status=batch.status)
+        paged.paged_attention(ctx, b["q_out"], A["cache"], batch.block_table, batch.kv_lens,
+                              b["out"], b["ws"], row_req=batch.token_req, status=batch.status)
+        return b["out"].view(cur.shape)
+
     def step(self) -> None:
         ctx, cur = self.ctx, self.x
+        if self.attn is not None:
+            self.kv.plan()
         for l, L in enumerate(self.layers):
             nxt = self.outs[l % 2]
-            if self.fuse_proj:
+            attn = L.get("attn")
+            if self.fuse_proj and attn is None:
                 # the next layer's router rows and projection codes into L2
                 # while this layer exchanges its act rows (its norm weights
                 # are read before the launch's dependency wait anyway)
@@ -119,7 +170,7 @@ class DecodeStack:
                                           self.ws, n_experts=self.E)
                 cur = nxt
                 continue
-            lfm.gemv_quant(ctx, L["proj"], cur, self.p)
+            lfm.gemv_quant(ctx, L["proj"], cur if attn is None else self._attend(attn, cur), self.p)
             if self.path == "fused":
                 following = self.layers[(l + 1) % len(self.layers)]
                 ctx.prefetch_next(following["router"], following["norm_w"])
@@ -140,13 +191,19 @@ class DecodeStack:
                     lfm.gemv_gather_down_combine4(ctx, L["down"], self.act, self.ids[l],
                                                   self.wts[l], nxt, n_experts=self.E)
             cur = nxt
-        if self.sample is None:
+        if self.head_logits is None:
             lfm.gemv_head_argmax(ctx, self.head, cur, self.keys)
         else:
             lfm.gemv_quant(ctx, self.head, cur, self.head_logits)
-            self.sample.encode_draw(self.head_logits, self.keys, self.sampling, self.pos)
+        if self.rules is not None:
+            logits_process(ctx, self.head_logits, self.head_logits, self.rules,
+                           self.keys if self.sample is None else None)
+        if self.sample is not None:
+            self.sample.encode_draw(self.head_logits[0], self.keys, self.sampling, self.pos)
         lfm.token_tail(ctx, self.keys, self.tokens,
                        (self.embed, self.tail_norm_w, self.x, self.tail_normed))
+        if self.rules is not None:
+            logits_mark(ctx, self.tokens, self.rules, self.head.out_features)
         if self.sample is not None:
             self.sample.encode_mark(self.tokens, self.pos)
 
@@ -167,6 +224,8 @@ class DecodeStack:
         run so far reported a wait that ran out (the tokens are then invalid)."""
         for w in self.status_words():
             lfm.raise_on_status(w, f"decode stack ({self.path})")
+        if self.attn is not None:
+            self.kv.check()
 
     def read_tokens(self) -> torch.Tensor:
         """The last step's tokens on the host, after check()."""
@@ -176,10 +235,15 @@ class DecodeStack:
     def launches_per_step(self) -> int:
         per_layer = {"fused": 1 if self.fuse_proj else 2, "gemv": 4,
                      "grouped": 2 + lfm.MOE_PREFILL_LAUNCHES}[self.path]
-        tail = 2
+        n = len(self.layers) * per_layer + 2
+        if self.attn is not None:
+            # norm, qkv, norm + rotation, attention, and the projection the fused layer leaves out
+            n_attn = sum("attn" in L for L in self.layers)
+            n += 1 + n_attn * (4 + self.fuse_proj)
+        if self.rules is not None:
+            n += 1 + (self.rules.seen is not None or self.rules.counts is not None)
         if self.sampling is not None:
             s = self.sampling
             full = (s.top_k == 0 or s.top_k >= self.head.out_features) and s.top_p >= 1.0
-            draw = 1 if full else 2 + 3 * ((s.top_k > 0) + (s.top_p < 1.0))
-            tail = 1 + draw + 1 + 1
-        return len(self.layers) * per_layer + tail
+            n += 1 + (1 if full else 2 + 3 * ((s.top_k > 0) + (s.top_p < 1.0)))
+        return n

@@ -232,3 +232,15 @@ def test_split_of_the_attention_work(tmp_path):
     assert r.returncode == 0, r.stderr
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.strip() == "ok (0 failures)", r.stdout
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_cpp_host_mirror_of_the_serving_calls(lib, tmp_path):
+    so = build.build()
+    exe = tmp_path / "serving"
+    r = subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Wextra", "-Werror", "-I", str(ROOT / "include"),
+                        str(ROOT / "tests" / "cpp" / "test_host_mirror_serving.cpp"), "-L", str(so.parent), "-lmolten_cuda",
+                        f"-Wl,-rpath,{so.parent}", "-o", str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and r.stdout.strip() == "ok (0 failures)", r.stdout
