@@ -187,13 +187,6 @@ __device__ __forceinline__ int v_dim(int nt, int n) {
   return 64 * (nt / 8) + 8 * n + nt % 8;
 }
 
-// Folds (m2, l2) into a running maximum and sum.
-__device__ __forceinline__ void fold(float& m, float& l, float m2, float l2) {
-  const float top = fmaxf(m, m2), use = top == -INFINITY ? 0.0f : top;
-  l = __fmaf_rn(l, ex2(m - use), ex2(m2 - use) * l2);
-  m = top;
-}
-
 template <int D, bool F8>
 __global__ void __launch_bounds__(Shape<D, F8>::kThreads, (Shape<D, F8>::kPerSm))
 paged_attention_kernel(const PaParams P) {
@@ -622,57 +615,95 @@ paged_attention_kernel(const PaParams P) {
     auto part_of = [&](int x) {
       return P.parts + part_floats(D) * (2 * (size_t)x + (x == first_cta ? 1 : 0));
     };
-    {  // the largest m and the sum, head tid % 8, pieces tid / 8, tid / 8 + threads / 8, ...
-      const int h = tid % kHeads;
-      float mx = -INFINITY, sum = 0.0f;
-      for (int x = first_cta + tid / kHeads; x <= last_cta; x += S::kThreads / kHeads) {
-        const float* pp = part_of(x) + kHeads * D + h;
-        fold(mx, sum, __ldcg(pp), __ldcg(pp + kHeads));
-      }
+    // Four elements a thread (or twice four), the pieces shared by `shares` threads for each, 12
+    // loads of them in flight; the shares' results meet in o_s, which is free here.
+    constexpr int kQ = kHeads * D / 4 > S::kThreads ? 2 : 1, kB = 12 / kQ;
+    static_assert(kQ * S::kThreads >= kHeads * D / 4, "a thread for each quad");
+    const int quads = heads * D / 4, shares = S::kThreads > quads ? S::kThreads / quads : 1;
+    const int share = tid / quads, at0 = shares > 1 ? tid % quads : tid;
+    float mx[kQ], sum[kQ];
+    float4 val[kQ];
 #pragma unroll
-      for (int d = kHeads; d < 32; d <<= 1)
-        fold(mx, sum, __shfl_xor_sync(0xffffffffu, mx, d), __shfl_xor_sync(0xffffffffu, sum, d));
-      if (lane < kHeads) {
-        m_s[warp][lane] = mx;
-        l_s[warp][lane] = sum;
-      }
+    for (int q = 0; q < kQ; ++q) {
+      mx[q] = -INFINITY;
+      sum[q] = 0.0f;
+      val[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    __syncthreads();
-    // four elements a thread, 8 pieces' loads in flight
-    for (int i = tid; i < heads * D / 4; i += S::kThreads) {
-      const int h = 4 * i / D;
-      float mx = -INFINITY, sum = 0.0f;
+    if (share < shares || shares == 1)
+      for (int x0 = first_cta + (shares > 1 ? share : 0); x0 <= last_cta; x0 += kB * shares) {
+        float4 v[kQ][kB];
+        float m8[kQ][kB], l8[kQ][kB];
 #pragma unroll
-      for (int y = 0; y < S::kWarps; ++y) fold(mx, sum, m_s[y][h], l_s[y][h]);
-      const float use = mx == -INFINITY ? 0.0f : mx;
-      float4 val = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (int x0 = first_cta; x0 <= last_cta; x0 += 8) {
-        float4 v[8];
-        float m8[8];
+        for (int k = 0; k < kB; ++k)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int x = x0 + k;
-          m8[k] = -INFINITY;
-          v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (x <= last_cta) {
-            v[k] = __ldcg(reinterpret_cast<const float4*>(part_of(x)) + i);
-            m8[k] = __ldcg(part_of(x) + kHeads * D + h);
+          for (int q = 0; q < kQ; ++q) {
+            const int x = x0 + k * shares, at = at0 + q * S::kThreads;
+            m8[q][k] = -INFINITY;
+            l8[q][k] = 0.0f;
+            v[q][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (x <= last_cta && at < quads) {
+              const float* pp = part_of(x);
+              v[q][k] = __ldcg(reinterpret_cast<const float4*>(pp) + at);
+              m8[q][k] = __ldcg(pp + kHeads * D + 4 * at / D);
+              l8[q][k] = __ldcg(pp + kHeads * D + kHeads + 4 * at / D);
+            }
+          }
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) {
+          float top = mx[q];
+#pragma unroll
+          for (int k = 0; k < kB; ++k) top = fmaxf(top, m8[q][k]);
+          const float use = top == -INFINITY ? 0.0f : top, a0 = ex2(mx[q] - use);
+          sum[q] *= a0;
+          val[q] = make_float4(val[q].x * a0, val[q].y * a0, val[q].z * a0, val[q].w * a0);
+          mx[q] = top;
+#pragma unroll
+          for (int k = 0; k < kB; ++k) {
+            const float a = ex2(m8[q][k] - use);
+            sum[q] = __fmaf_rn(a, l8[q][k], sum[q]);
+            val[q].x = __fmaf_rn(a, v[q][k].x, val[q].x);
+            val[q].y = __fmaf_rn(a, v[q][k].y, val[q].y);
+            val[q].z = __fmaf_rn(a, v[q][k].z, val[q].z);
+            val[q].w = __fmaf_rn(a, v[q][k].w, val[q].w);
           }
         }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float a = ex2(m8[k] - use);
-          val.x = __fmaf_rn(a, v[k].x, val.x);
-          val.y = __fmaf_rn(a, v[k].y, val.y);
-          val.z = __fmaf_rn(a, v[k].z, val.z);
-          val.w = __fmaf_rn(a, v[k].w, val.w);
-        }
       }
-      const int d = 4 * i % D;
-      finish(row, head0 + h, kvh, d, mx, sum, val.x);
-      finish(row, head0 + h, kvh, d + 1, mx, sum, val.y);
-      finish(row, head0 + h, kvh, d + 2, mx, sum, val.z);
-      finish(row, head0 + h, kvh, d + 3, mx, sum, val.w);
+    auto finish4 = [&](int at, float m, float l, const float4& v) {
+      const int h = head0 + 4 * at / D, d = 4 * at % D;
+      finish(row, h, kvh, d, m, l, v.x);
+      finish(row, h, kvh, d + 1, m, l, v.y);
+      finish(row, h, kvh, d + 2, m, l, v.z);
+      finish(row, h, kvh, d + 3, m, l, v.w);
+    };
+    if (shares == 1) {
+#pragma unroll
+      for (int q = 0; q < kQ; ++q)
+        if (at0 + q * S::kThreads < quads) finish4(at0 + q * S::kThreads, mx[q], sum[q], val[q]);
+      continue;
+    }
+    float* stats = o_s + 4 * S::kThreads;
+    if (share < shares) {
+      reinterpret_cast<float4*>(o_s)[tid] = val[0];
+      stats[2 * tid] = mx[0];
+      stats[2 * tid + 1] = sum[0];
+    }
+    __syncthreads();
+    if (tid < quads) {
+      float top = -INFINITY, total = 0.0f;
+      for (int k = 0; k < shares; ++k) top = fmaxf(top, stats[2 * (tid + k * quads)]);
+      const float use = top == -INFINITY ? 0.0f : top;
+      float4 o4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int k = 0; k < shares; ++k) {
+        const int j = tid + k * quads;
+        const float a = ex2(stats[2 * j] - use);
+        const float4 u = reinterpret_cast<const float4*>(o_s)[j];
+        total = __fmaf_rn(a, stats[2 * j + 1], total);
+        o4.x = __fmaf_rn(a, u.x, o4.x);
+        o4.y = __fmaf_rn(a, u.y, o4.y);
+        o4.z = __fmaf_rn(a, u.z, o4.z);
+        o4.w = __fmaf_rn(a, u.w, o4.w);
+      }
+      finish4(tid, top, total, o4);
     }
   } while (ps_next(piece, P.items, P.rows, units_of));
   if (gave_up) {  // copies still on their way end before the shared memory goes

@@ -62,8 +62,14 @@ PS_HD int ps_units(PsRow r, int unit) {
   return n <= unit ? 1 : (int)(((long long)n + unit - 1) / unit);
 }
 
-// floor(U c / G) without the wide product.
-PS_HD long long ps_begin(long long U, int c, int G) { return U / G * c + U % G * c / G; }
+// floor(U c / G) without the wide product (32-bit divisions where U allows).
+PS_HD long long ps_begin(long long U, int c, int G) {
+  if (U <= 0x7fffffff) {
+    const uint32_t q = (uint32_t)U / (uint32_t)G, r = (uint32_t)U - q * (uint32_t)G;  // r c < 2^20
+    return (long long)q * c + r * (uint32_t)c / (uint32_t)G;
+  }
+  return U / G * c + U % G * c / G;
+}
 
 // The CTA whose range holds unit u (0 <= u < U, G <= U).
 PS_HD int ps_owner(long long u, long long U, int G) {
@@ -86,7 +92,8 @@ PS_HD PsCursor ps_first(int row, long long in_row, int n, int items, long long l
   PsCursor c;
   c.row = row;
   c.n = n;
-  const long long item = in_row / n;
+  const long long item =
+      in_row <= 0x7fffffff ? (long long)((uint32_t)in_row / (uint32_t)n) : in_row / n;
   c.item = item < items ? (int)item : items - 1;
   c.unit = item < items ? (int)(in_row - item * n) : n - 1;
   c.left = left;
