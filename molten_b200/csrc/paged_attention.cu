@@ -72,6 +72,8 @@ struct PaParams {
   const float* v_scale;
   const int32_t* table;
   int n_req, width;
+  int capacity;    // keys the table can hold, clear of the int range's end
+  int small_unit;  // ps_small_unit
   const int32_t* kv_lens;
   const int32_t* row_req;
   int window;
@@ -167,7 +169,7 @@ struct Shape {
   static constexpr int kStages = kRow == 64 ? 4 : D == 64 ? 3 : 2;
   static constexpr int kPerSm = kRow == 64 ? 3 : 2;  // CTAs an SM holds at once
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kUnit = kWarps * kStep;    // keys of a unit
+  static constexpr int kUnit = kWarps * kStep;    // keys of a (small) unit
   static constexpr int kORow = D + 4;             // floats of a row in o
   static constexpr size_t kRingBytes = (size_t)kWarps * kStages * kStage;
   static constexpr size_t kOBytes = (size_t)kWarps * kHeads * kORow * sizeof(float);
@@ -201,17 +203,14 @@ paged_attention_kernel(const PaParams P) {
   __shared__ __align__(8) uint64_t full_s[S::kWarps][S::kStages];
   __shared__ uint32_t live_s[S::kWarps][S::kStages];
   __shared__ float m_s[S::kWarps][kHeads], l_s[S::kWarps][kHeads];
-  __shared__ long long sums_s[S::kWarps];
-  __shared__ long long in_row_s;
-  __shared__ int row_s;
   __shared__ uint32_t last_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid < S::kWarps * S::kStages) mc_mbar_init(&full_s[0][0] + tid, 32);
+  if (lane < S::kStages) mc_mbar_init(&full_s[warp][lane], 32);  // a warp's own
   mc_fence_barrier_init();
+  __syncwarp();
   mc_pdl_launch_dependents();
   mc_pdl_wait();
-  // keys the table can hold; key indices stay clear of the int range's end
-  const long long capacity = min((long long)P.width * P.block_size, 0x7fff0000ll);
+  const int capacity = P.capacity;
   const int cta = blockIdx.x;
 
   auto row_of = [&](int r) {
@@ -222,53 +221,64 @@ paged_attention_kernel(const PaParams P) {
     }
     return ps_row(len, capacity, P.window);
   };
-  auto units_of = [&](int r) { return ps_units(row_of(r), S::kUnit); };
+  int unit = P.small_unit;  // keys of a unit
+  auto units_of = [&](int r) { return ps_units(row_of(r), unit); };
 
-  // ---- this CTA's range of units, and the row it starts in
-  const int per = (P.rows + S::kThreads - 1) / S::kThreads;
-  const int r_lo = min(tid * per, P.rows), r_hi = min(r_lo + per, P.rows);
-  long long mine = 0;
-  for (int r = r_lo; r < r_hi; ++r) {
-    mine += (long long)units_of(r) * P.items;
-    if (cta == 0 && P.status) {
+  // ---- this CTA's range of units, and the row it starts in. Every warp finds them for itself:
+  // a run of rows a lane, no barrier.
+  const int per = (P.rows + 31) / 32;
+  const int r_lo = min(lane * per, P.rows), r_hi = min(r_lo + per, P.rows);
+  int mine, incl, U;  // units of this lane's rows, up to and with them, of all rows
+  int n_max;
+  auto scan = [&]() {
+    mine = 0;
+    n_max = 0;
+    for (int r = r_lo; r < r_hi; ++r) {
+      const int n = units_of(r);
+      mine += n * P.items;
+      n_max = max(n_max, n);
+    }
+    incl = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += o;
+    }
+    U = __shfl_sync(0xffffffffu, incl, 31);
+    n_max = __reduce_max_sync(0xffffffffu, n_max);
+  };
+  scan();
+  const int factor = ps_factor(U, n_max, P.rows * P.items, gridDim.x);
+  if (factor > 1) {
+    unit = (int)min((long long)unit * factor, 0x7fffffffll);
+    scan();
+  }
+  if (cta == 0 && warp == 0 && P.status)
+    for (int r = r_lo; r < r_hi; ++r) {
       if (P.kv_lens[r] < 0 || P.kv_lens[r] > capacity) atomicOr(P.status, MC_KV_BAD_LENGTH);
       if (P.row_req && (P.row_req[r] < -1 || P.row_req[r] >= P.n_req))
         atomicOr(P.status, MC_KV_BAD_ROW);
     }
-  }
-  long long incl = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const long long o = __shfl_up_sync(0xffffffffu, incl, d);
-    if (lane >= d) incl += o;
-  }
-  if (lane == 31) sums_s[warp] = incl;
-  __syncthreads();
-  long long U = 0;
-#pragma unroll
-  for (int w = 0; w < S::kWarps; ++w) {
-    if (w < warp) incl += sums_s[w];
-    U += sums_s[w];
-  }
-  const int G = (int)min((long long)gridDim.x, U);
+  const int G = min((int)gridDim.x, U);
   if (cta >= G) return;
-  const long long u0 = ps_begin(U, cta, G), u_end = ps_begin(U, cta + 1, G);
-  if (u0 >= incl - mine && u0 < incl) {
-    long long at = incl - mine;
-    int r = r_lo;
-    for (; r < r_hi - 1; ++r) {
-      const long long n = (long long)units_of(r) * P.items;
-      if (u0 < at + n) break;
-      at += n;
+  const int u0 = ps_begin(U, cta, G), u_end = ps_begin(U, cta + 1, G);
+  int row_at = incl - mine;
+  int row0 = r_lo;
+  const bool here = u0 >= row_at && u0 < incl;
+  if (here) {
+    for (; row0 < r_hi - 1; ++row0) {
+      const int n = units_of(row0) * P.items;
+      if (u0 < row_at + n) break;
+      row_at += n;
     }
-    row_s = r;
-    in_row_s = u0 - at;
   }
-  __syncthreads();
+  const int owner = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+  row0 = __shfl_sync(0xffffffffu, row0, owner);
+  row_at = __shfl_sync(0xffffffffu, row_at, owner);
 
   // ---- filling the ring: the step at fill_base of the piece `fill`
   uint8_t* ring = ring_s + (size_t)warp * S::kStages * S::kStage;
-  PsCursor fill = ps_first(row_s, in_row_s, units_of(row_s), P.items, u_end - u0);
+  PsCursor fill = ps_first(row0, u0 - row_at, units_of(row0), P.items, u_end - u0);
   PsCursor piece = fill;
   int fill_base = 0, fill_hi = 0, fill_stage = 0, page = -1;
   uint32_t filled = 0, in_page = 0, head_row = 0;
@@ -276,8 +286,8 @@ paged_attention_kernel(const PaParams P) {
   const int32_t* table = nullptr;
   auto enter = [&]() {  // the piece `fill`
     const PsRow keys = row_of(fill.row);
-    const int lo = keys.low + fill.unit * S::kUnit;
-    fill_hi = (int)min((long long)keys.len, (long long)lo + (long long)fill.units * S::kUnit);
+    const int lo = keys.low + fill.unit * unit;
+    fill_hi = (int)min((long long)keys.len, (long long)lo + (long long)fill.units * unit);
     fill_base = lo + warp * S::kStep;
     head_row = (uint32_t)(fill.item / P.subs) * P.block_size;
     table = P.table + (size_t)(P.row_req ? max(P.row_req[fill.row], 0) : fill.row) * P.width;
@@ -357,8 +367,8 @@ paged_attention_kernel(const PaParams P) {
     const int row = piece.row;
     const int kvh = piece.item / P.subs, sub = piece.item - kvh * P.subs;
     const int head0 = kvh * P.group + sub * kHeads, heads = min(kHeads, P.group - sub * kHeads);
-    const int lo = keys.low + piece.unit * S::kUnit;
-    const int hi = (int)min((long long)keys.len, (long long)lo + (long long)piece.units * S::kUnit);
+    const int lo = keys.low + piece.unit * unit;
+    const int hi = (int)min((long long)keys.len, (long long)lo + (long long)piece.units * unit);
 
     // ---- Q: row lane/4 of the tile (heads past the item's are zero)
     uint32_t qa[D / 16][2];
@@ -599,7 +609,7 @@ paged_attention_kernel(const PaParams P) {
     }
     if (begins && ends) continue;
     // ---- the last of the item's CTAs joins the pieces in order
-    const long long first_unit = u_end - piece.left - piece.unit;
+    const int first_unit = u_end - piece.left - piece.unit;
     const int first_cta = begins ? cta : ps_owner(first_unit, U, G);
     const int last_cta = ends ? cta : ps_owner(first_unit + piece.n - 1, U, G);
     __syncthreads();
@@ -713,13 +723,16 @@ paged_attention_kernel(const PaParams P) {
 }
 
 template <int D, bool F8>
-int launch_attention(mc_ctx* ctx, const PaParams& P) {
+int launch_attention(mc_ctx* ctx, PaParams& P) {
   using S = Shape<D, F8>;
+  const long long items = (long long)P.rows * P.items;
+  P.small_unit = ps_small_unit(S::kUnit, items, P.capacity);
+  if (P.small_unit == 0)
+    return mc_fail(MC_EUNSUPPORTED, "paged_attention: %lld row and head groups", items);
   auto fn = paged_attention_kernel<D, F8>;
   MC_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
   long long g = (long long)ctx->num_sms * S::kPerSm;
-  const long long most =
-      (((long long)P.width * P.block_size + S::kUnit - 1) / S::kUnit) * P.rows * P.items;
+  const long long most = ((long long)P.capacity + S::kUnit - 1) / S::kUnit * items;
   if (g > most) g = most;
   if (g > kMaxCtas) g = kMaxCtas;
   MC_CUDA(mc_launch_pdl(fn, dim3((unsigned)g), dim3(S::kThreads), S::kSmem, ctx->stream, P));
@@ -774,9 +787,11 @@ extern "C" int mc_paged_attention(mc_ctx* ctx, const uint16_t* q, size_t q_strid
   McDeviceGuard dev(ctx->device);
   MC_CUDA(dev.error());
   const int group = n_heads / n_kv_heads, subs = (group + kHeads - 1) / kHeads;
-  const PaParams P{q, q_stride, n_rows, n_heads, n_kv_heads, group, subs, n_kv_heads * subs,
+  const long long capacity = (long long)table_width * block_size;
+  PaParams P{q, q_stride, n_rows, n_heads, n_kv_heads, group, subs, n_kv_heads * subs,
                    k_cache, v_cache, num_blocks, block_size, (uint32_t)(block_stride / head_dim),
-                   ps_div_of(block_size), k_scale, v_scale, block_table, n_req, table_width, kv_lens, row_req, window, scale * kLog2e,
+                   ps_div_of(block_size), k_scale, v_scale, block_table, n_req, table_width,
+             (int)(capacity < 0x7fff0000ll ? capacity : 0x7fff0000ll), 0, kv_lens, row_req, window, scale * kLog2e,
                    out, out_stride, lse, static_cast<uint32_t*>(workspace),
                    reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes), status,
                    mc_wait_limit(ctx, 1000000000ull)};

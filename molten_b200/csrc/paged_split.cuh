@@ -8,7 +8,10 @@
 // out evenly: CTA c of G takes units [U c / G, U (c + 1) / G). A CTA's range
 // is a run of pieces, one for each item it touches; an item whole inside one
 // CTA is written at once, one that spans several CTAs is joined from their
-// partial results.
+// partial results. Where the items are alike enough, the unit is made so long
+// that every CTA has one piece (ps_factor). The host chooses the smallest unit
+// so that there are fewer than 2^31 (ps_small_unit): the arithmetic is in 32
+// bits.
 #pragma once
 #include <stdint.h>
 
@@ -49,31 +52,55 @@ struct PsRow {
 };
 
 // len clamped to [0, capacity]; a window keeps the last `window` keys (0: all).
-PS_HD PsRow ps_row(int len, long long capacity, int window) {
+PS_HD PsRow ps_row(int len, int capacity, int window) {
   PsRow r;
-  r.len = len < 0 ? 0 : (long long)len > capacity ? (int)capacity : len;
+  r.len = len < 0 ? 0 : len > capacity ? capacity : len;
   r.low = window > 0 && r.len > window ? r.len - window : 0;
   return r;
 }
 
-// Units of one item of a row.
+// Units of one item of a row (unit < 2^31).
 PS_HD int ps_units(PsRow r, int unit) {
-  const int n = r.len - r.low;
-  return n <= unit ? 1 : (int)(((long long)n + unit - 1) / unit);
+  const uint32_t n = (uint32_t)(r.len - r.low);
+  return n <= (uint32_t)unit ? 1 : (int)((n + (uint32_t)unit - 1) / (uint32_t)unit);
 }
 
-// floor(U c / G) without the wide product (32-bit divisions where U allows).
-PS_HD long long ps_begin(long long U, int c, int G) {
-  if (U <= 0x7fffffff) {
-    const uint32_t q = (uint32_t)U / (uint32_t)G, r = (uint32_t)U - q * (uint32_t)G;  // r c < 2^20
-    return (long long)q * c + r * (uint32_t)c / (uint32_t)G;
+// The smallest unit, `unit` times a power of two, with which `items` items of
+// up to `capacity` keys have fewer than 2^31 units; 0: none.
+inline int ps_small_unit(int unit, long long items, int capacity) {
+  for (long long u = unit; u < 0x40000000; u *= 2) {
+    const long long n = ((long long)capacity + u - 1) / u;
+    if (items <= 0x7fffffffll / (n < 1 ? 1 : n)) return (int)u;
   }
-  return U / G * c + U % G * c / G;
+  return 0;
+}
+
+// How many small units make the unit. Let U small units, at most n_max in an
+// item, `items` items and `slots` CTAs. With f = ceil(n_max / (slots / items))
+// no item has more than slots / items units, so each CTA gets one unit at
+// most: no CTA works at two items and fewer items are joined, but the longest
+// CTA has f small units instead of U / slots. A second piece in a CTA and a
+// join cost as much as two or three small units, so f is taken while it is at
+// most 2 above the even share; and items of up to 3 small units stay whole.
+// (32 rows of 300 keys, 8 KV heads: 14.4 us without, 8.3 us; 8 rows of 2048:
+// 16.5 us, 14.1 us.)
+PS_HD int ps_factor(int U, int n_max, int items, int slots) {
+  if (items > slots) return 1;
+  if (n_max <= 3) return n_max;
+  const int p = slots / items;
+  const int f = (int)((uint32_t)(n_max + p - 1) / (uint32_t)p);
+  return (f - 2) * slots <= U ? f : 1;  // (f - 2) slots < 2 n_max items + slots
+}
+
+// floor(U c / G), G <= 1024, 0 <= c <= G.
+PS_HD int ps_begin(int U, int c, int G) {
+  const uint32_t q = (uint32_t)U / (uint32_t)G, r = (uint32_t)U - q * (uint32_t)G;  // r c <= 2^20
+  return (int)(q * (uint32_t)c + r * (uint32_t)c / (uint32_t)G);
 }
 
 // The CTA whose range holds unit u (0 <= u < U, G <= U).
-PS_HD int ps_owner(long long u, long long U, int G) {
-  const long long c = ((u + 1) * G - 1) / U;
+PS_HD int ps_owner(int u, int U, int G) {
+  const long long c = (((long long)u + 1) * G - 1) / U;
   return c < 0 ? 0 : c < G ? (int)c : G - 1;
 }
 
@@ -83,21 +110,20 @@ struct PsCursor {
   int row, item;    // query row, item within the row
   int n;            // units of each of the row's items
   int unit, units;  // first unit of the piece within the item, unit count
-  long long left;
+  int left;
 };
 
 // The piece that starts `in_row` units after the start of row `row` (n units
 // an item), with `left` units of the range to go.
-PS_HD PsCursor ps_first(int row, long long in_row, int n, int items, long long left) {
+PS_HD PsCursor ps_first(int row, int in_row, int n, int items, int left) {
   PsCursor c;
   c.row = row;
   c.n = n;
-  const long long item =
-      in_row <= 0x7fffffff ? (long long)((uint32_t)in_row / (uint32_t)n) : in_row / n;
-  c.item = item < items ? (int)item : items - 1;
-  c.unit = item < items ? (int)(in_row - item * n) : n - 1;
+  const int item = (int)((uint32_t)in_row / (uint32_t)n);
+  c.item = item < items ? item : items - 1;
+  c.unit = item < items ? in_row - item * n : n - 1;
   c.left = left;
-  c.units = left < n - c.unit ? (int)left : n - c.unit;
+  c.units = left < n - c.unit ? left : n - c.unit;
   return c;
 }
 
@@ -115,6 +141,6 @@ PS_HD bool ps_next(PsCursor& c, int items, int rows, F&& units_of) {
     if (++c.row >= rows) return false;
     c.n = units_of(c.row);
   }
-  c.units = c.left < c.n ? (int)c.left : c.n;
+  c.units = c.left < c.n ? c.left : c.n;
   return true;
 }

@@ -21,26 +21,40 @@ static int failures = 0;
     }                                                        \
   } while (0)
 
-static void run(const std::vector<int>& lens, long long capacity, int window, int items, int grid,
+static void run(const std::vector<int>& lens, int capacity, int window, int items, int grid,
                 int unit) {
   const int R = (int)lens.size();
-  long long U = 0;
-  for (int r = 0; r < R; ++r) U += (long long)ps_units(ps_row(lens[r], capacity, window), unit) * items;
-  const int G = (int)std::min<long long>(grid, U);
+  unit = ps_small_unit(unit, (long long)R * items, capacity);
+  CHECK(unit > 0);
+  long long sum = 0;
+  int n_max = 0;
+  for (int r = 0; r < R; ++r) {
+    const int n = ps_units(ps_row(lens[r], capacity, window), unit);
+    sum += (long long)n * items;
+    n_max = std::max(n_max, n);
+  }
+  CHECK(sum <= 0x7fffffff);
+  const int f = ps_factor((int)sum, n_max, R * items, grid);
+  CHECK(f >= 1 && (f == 1 || f <= n_max));
+  const bool one_each = f > 1 || ((long long)R * items <= grid && n_max <= 3);
+  unit = (int)std::min<long long>((long long)unit * f, 0x7fffffff);
+  int U = 0;
+  for (int r = 0; r < R; ++r) U += ps_units(ps_row(lens[r], capacity, window), unit) * items;
+  const int G = std::min(grid, U);
   auto units_of = [&](int r) {
     CHECK(r < R);
     return ps_units(ps_row(lens[r], capacity, window), unit);
   };
   std::map<std::pair<int, int>, std::vector<std::pair<int, PsCursor>>> of;  // item -> (cta, piece)
-  long long covered = 0;
+  int covered = 0;
   for (int c = 0; c < G; ++c) {
-    const long long u0 = ps_begin(U, c, G), u_end = ps_begin(U, c + 1, G);
+    const int u0 = ps_begin(U, c, G), u_end = ps_begin(U, c + 1, G);
     CHECK(u0 < u_end);
     CHECK(ps_owner(u0, U, G) == c && ps_owner(u_end - 1, U, G) == c);
     int row = 0;
-    long long start = 0;
+    int start = 0;
     for (;;) {
-      const long long n = (long long)units_of(row) * items;
+      const int n = units_of(row) * items;
       if (u0 < start + n) break;
       start += n;
       ++row;
@@ -52,7 +66,7 @@ static void run(const std::vector<int>& lens, long long capacity, int window, in
       CHECK(p.n == units_of(p.row) && p.left == u_end - u0 - (covered - u0));
       const bool begins = p.unit == 0, ends = p.unit + p.units == p.n;
       // what the kernel asks of an item that is not whole in this CTA
-      const long long u = u_end - p.left;
+      const int u = u_end - p.left;
       CHECK((ps_owner(u - p.unit, U, G) == c) == begins);
       CHECK((ps_owner(u - p.unit + p.n - 1, U, G) == c) == ends);
       if (!(begins && ends)) (begins ? continued : joined_in)++;
@@ -61,6 +75,7 @@ static void run(const std::vector<int>& lens, long long capacity, int window, in
     } while (ps_next(p, items, R, units_of));
     CHECK(covered == u_end);
     CHECK(continued <= 1 && joined_in <= 1);
+    if (one_each) CHECK(u_end - u0 == 1);
   }
   CHECK(covered == U);
   CHECK((long long)of.size() == (long long)R * items);
@@ -99,7 +114,9 @@ int main() {
   run({0}, 16, 0, 1, 444, 64);
   run({1}, 16, 0, 8, 444, 64);
   run({131072}, 131072, 0, 8, 444, 64);
-  run({0x7fffffff}, 0x7fff0000ll, 0, 1, 1024, 64);
+  run({0x7fffffff}, 0x7fff0000, 0, 1, 1024, 64);
+  run(std::vector<int>(300, 0x7fffffff), 0x7fff0000, 0, 9, 1024, 64);
+  CHECK(ps_small_unit(64, 1ll << 40, 1) == 0);
   run({-5, 70000, 0, 65}, 1 << 20, 0, 3, 296, 64);
   run(std::vector<int>(65, 64), 1 << 20, 0, 2, 7, 64);
   for (int i = 0; i < 400; ++i) {
