@@ -174,7 +174,8 @@ struct Shape {
   static constexpr size_t kRingBytes = (size_t)kWarps * kStages * kStage;
   static constexpr size_t kOBytes = (size_t)kWarps * kHeads * kORow * sizeof(float);
   static constexpr size_t kSmem = kRingBytes + kOBytes;
-  static_assert(kPerSm * (kSmem + 2048) <= 228 * 1024, "shared memory");
+  // a CTA has some 0.5 KB of static shared memory too, and the system takes 1 KB of each
+  static_assert(kPerSm * (kSmem + 1536) <= 228 * 1024, "shared memory");
 };
 
 __device__ __forceinline__ uint32_t word(const uint4& u, int i) {
@@ -355,80 +356,88 @@ paged_attention_kernel(const PaParams P) {
   const int v_at = S::kPart * c * S::kRow +
                    (kHalfChunk ? 16 * ((hr >> 1) ^ (2 * c)) + 8 * (hr & 1) : 16 * (hr ^ (2 * c)));
   const int v_flip = (v_at ^ 64) - v_at;
-  auto finish = [&](int row, int head, int kvh, int d, float mx, float sum, float val) {
-    const float vscale = F8 && P.v_scale ? P.v_scale[kvh] : 1.0f;
-    const float r = sum == 0.0f ? 0.0f : __fdiv_rn(val, sum) * vscale;
-    P.out[(size_t)row * P.out_stride + (size_t)head * D + d] = mc_f32_to_bf16(r);
+  // Four elements of an item's result (quad `at`: head 4 at / D of the item) from their sums.
+  auto finish = [&](int row, int head0, float vscale, int at, float mx, float sum, const float4& v) {
+    const int head = head0 + 4 * at / D, d = 4 * at % D;
+    const float by = sum == 0.0f ? 0.0f : __fdiv_rn(vscale, sum);  // NaN of a zero sum: 0
+    uint2 r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r.x) : "f"(v.y * by), "f"(v.x * by));
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r.y) : "f"(v.w * by), "f"(v.z * by));
+    *reinterpret_cast<uint2*>(P.out + (size_t)row * P.out_stride + (size_t)head * D + d) = r;
     if (P.lse && d == 0)
       P.lse[(size_t)row * P.H + head] = sum == 0.0f ? -INFINITY : __fmaf_rn(mx, kLn2, logf(sum));
   };
-  do {
+  // A piece's queries, as stored: row lane/4 of the tile (heads past the item's are zero), bf16
+  // dims 8 (c + 4 i), e4m3 16 c + 64 (i / 2) + 8 (i % 2). They are asked for while the piece before
+  // is merged, when its sums have left the registers.
+  uint4 q_raw[D / 32];
+  auto load_q = [&](const PsCursor& p) {
+    const int kvh = p.item / P.subs, sub = p.item - kvh * P.subs, h = sub * kHeads + hr;
+    const uint4* q = reinterpret_cast<const uint4*>(P.q + (size_t)p.row * P.q_stride +
+                                                    (size_t)(kvh * P.group + h) * D);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      q_raw[i] = make_uint4(0, 0, 0, 0);
+      if (h < P.group) q_raw[i] = __ldg(q + (F8 ? 2 * c + 8 * (i / 2) + i % 2 : c + 4 * i));
+    }
+  };
+  load_q(piece);
+  for (bool more_pieces = true; more_pieces;) {
     const PsRow keys = row_of(piece.row);
     const int row = piece.row;
     const int kvh = piece.item / P.subs, sub = piece.item - kvh * P.subs;
     const int head0 = kvh * P.group + sub * kHeads, heads = min(kHeads, P.group - sub * kHeads);
     const int lo = keys.low + piece.unit * unit;
     const int hi = (int)min((long long)keys.len, (long long)lo + (long long)piece.units * unit);
+    const float vscale = F8 && P.v_scale ? P.v_scale[kvh] : 1.0f;
 
-    // ---- Q: row lane/4 of the tile (heads past the item's are zero)
+    // ---- Q's fragments
     uint32_t qa[D / 16][2];
     float qk = P.scale_log2;
-    {
-      const uint16_t* q = P.q + (size_t)row * P.q_stride + (size_t)(head0 + hr) * D;
-      if (!F8) {
+    if (!F8) {
 #pragma unroll
-        for (int i = 0; i < kKLoads; ++i) {
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (hr < heads) w = __ldg(reinterpret_cast<const uint4*>(q) + c + 4 * i);
-          qa[2 * i][0] = w.x;
-          qa[2 * i][1] = w.y;
-          qa[2 * i + 1][0] = w.z;
-          qa[2 * i + 1][1] = w.w;
+      for (int i = 0; i < kKLoads; ++i) {
+        qa[2 * i][0] = q_raw[i].x;
+        qa[2 * i][1] = q_raw[i].y;
+        qa[2 * i + 1][0] = q_raw[i].z;
+        qa[2 * i + 1][1] = q_raw[i].w;
+      }
+    } else {
+      float f[D / 4];
+      float top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float2 p = unpack2<false>(word(q_raw[i], x));
+          f[8 * i + 2 * x] = p.x;
+          f[8 * i + 2 * x + 1] = p.y;
+          top = fmaxf(top, fmaxf(fabsf(p.x), fabsf(p.y)));
         }
-      } else {
-        // dims 16 (lane%4) + 64 i + 0..15: two 16-byte loads for each K load
-        float f[D / 4];
-        float top = 0.0f;
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^-e with 2^e <= top < 2^(e+1); 1 for zero, subnormal or infinite rows
+      const int e = (int)(__float_as_uint(top) >> 23) - 127;
+      const bool plain = e < -126 || e > 126;
+      const float down = plain ? 1.0f : __uint_as_float((uint32_t)(127 - e) << 23);
+      const float up = plain ? 1.0f : __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
-        for (int i = 0; i < kKLoads; ++i)
+      for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (hr < heads) w = __ldg(reinterpret_cast<const uint4*>(q) + 2 * c + 8 * i + z);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const float2 p = unpack2<false>(word(w, x));
-              f[16 * i + 8 * z + 2 * x] = p.x;
-              f[16 * i + 8 * z + 2 * x + 1] = p.y;
-              top = fmaxf(top, fmaxf(fabsf(p.x), fabsf(p.y)));
-            }
-          }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // 2^-e with 2^e <= top < 2^(e+1); 1 for zero, subnormal or infinite rows
-        const int e = (int)(__float_as_uint(top) >> 23) - 127;
-        const bool plain = e < -126 || e > 126;
-        const float down = plain ? 1.0f : __uint_as_float((uint32_t)(127 - e) << 23);
-        const float up = plain ? 1.0f : __uint_as_float((uint32_t)(127 + e) << 23);
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-            qa[i][x] = pack2<true>(f[4 * i + 2 * x] * down, f[4 * i + 2 * x + 1] * down);
-        qk *= up;
-        if (P.k_scale) qk *= P.k_scale[kvh];
-      }
-      // a factor above zero keeps the order of the scores (and -inf times it is -inf)
-      if (qk < 0.0f) {
-        qk = -qk;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) qa[i][x] ^= 0x80008000u;
-      }
-      qk = fmaxf(qk, 1e-37f);
+        for (int x = 0; x < 2; ++x)
+          qa[i][x] = pack2<true>(f[4 * i + 2 * x] * down, f[4 * i + 2 * x + 1] * down);
+      qk *= up;
+      if (P.k_scale) qk *= P.k_scale[kvh];
     }
-
+    // a factor above zero keeps the order of the scores (and -inf times it is -inf)
+    if (qk < 0.0f) {
+      qk = -qk;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) qa[i][x] ^= 0x80008000u;
+    }
+    qk = fmaxf(qk, 1e-37f);
     float o[kT][4];
 #pragma unroll
     for (int i = 0; i < kT; ++i)
@@ -581,26 +590,34 @@ paged_attention_kernel(const PaParams P) {
         *reinterpret_cast<float4*>(o_s + (warp * kHeads + hr) * S::kORow + v_dim<D, F8>(i, 2 * c + x)) =
             make_float4(o[i][x] + o[i][x + 2], o[i + 1][x] + o[i + 1][x + 2],
                         o[i + 2][x] + o[i + 2][x + 2], o[i + 3][x] + o[i + 3][x + 2]);
-    __syncthreads();
     const bool begins = piece.unit == 0, ends = piece.unit + piece.units == piece.n;
+    const int n_units = piece.n, first_unit = u_end - piece.left - piece.unit;
+    more_pieces = ps_next(piece, P.items, P.rows, units_of);
+    if (more_pieces) load_q(piece);
+    __syncthreads();
     float* part = P.parts + part_floats(D) * (2 * (size_t)cta + (begins ? 1 : 0));
-    for (int i = tid; i < kHeads * D; i += S::kThreads) {
-      const int h = i / D, d = i % D;
+    for (int at = tid; at < heads * D / 4; at += S::kThreads) {
+      const int h = 4 * at / D, d = 4 * at % D;
       float mx = m_s[0][h];
 #pragma unroll
       for (int w = 1; w < S::kWarps; ++w) mx = fmaxf(mx, m_s[w][h]);
       const float use = mx == -INFINITY ? 0.0f : mx;
-      float sum = 0.0f, val = 0.0f;
+      float sum = 0.0f;
+      float4 val = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int w = 0; w < S::kWarps; ++w) {
         const float a = ex2(m_s[w][h] - use);
+        const float4 u = *reinterpret_cast<const float4*>(o_s + (w * kHeads + h) * S::kORow + d);
         sum = __fmaf_rn(a, l_s[w][h], sum);
-        val = __fmaf_rn(a, o_s[(w * kHeads + h) * S::kORow + d], val);
+        val.x = __fmaf_rn(a, u.x, val.x);
+        val.y = __fmaf_rn(a, u.y, val.y);
+        val.z = __fmaf_rn(a, u.z, val.z);
+        val.w = __fmaf_rn(a, u.w, val.w);
       }
       if (begins && ends) {
-        if (h < heads) finish(row, head0 + h, kvh, d, mx, sum, val);
+        finish(row, head0, vscale, at, mx, sum, val);
       } else {
-        part[i] = val;
+        reinterpret_cast<float4*>(part)[at] = val;
         if (d == 0) {
           part[kHeads * D + h] = mx;
           part[kHeads * D + kHeads + h] = sum;
@@ -609,9 +626,8 @@ paged_attention_kernel(const PaParams P) {
     }
     if (begins && ends) continue;
     // ---- the last of the item's CTAs joins the pieces in order
-    const int first_unit = u_end - piece.left - piece.unit;
     const int first_cta = begins ? cta : ps_owner(first_unit, U, G);
-    const int last_cta = ends ? cta : ps_owner(first_unit + piece.n - 1, U, G);
+    const int last_cta = ends ? cta : ps_owner(first_unit + n_units - 1, U, G);
     __syncthreads();
     if (tid == 0) {
       __threadfence();  // this CTA's part, written before the barrier
@@ -678,17 +694,11 @@ paged_attention_kernel(const PaParams P) {
           }
         }
       }
-    auto finish4 = [&](int at, float m, float l, const float4& v) {
-      const int h = head0 + 4 * at / D, d = 4 * at % D;
-      finish(row, h, kvh, d, m, l, v.x);
-      finish(row, h, kvh, d + 1, m, l, v.y);
-      finish(row, h, kvh, d + 2, m, l, v.z);
-      finish(row, h, kvh, d + 3, m, l, v.w);
-    };
     if (shares == 1) {
 #pragma unroll
       for (int q = 0; q < kQ; ++q)
-        if (at0 + q * S::kThreads < quads) finish4(at0 + q * S::kThreads, mx[q], sum[q], val[q]);
+        if (at0 + q * S::kThreads < quads) 
+          finish(row, head0, vscale, at0 + q * S::kThreads, mx[q], sum[q], val[q]);
       continue;
     }
     float* stats = o_s + 4 * S::kThreads;
@@ -713,9 +723,9 @@ paged_attention_kernel(const PaParams P) {
         o4.z = __fmaf_rn(a, u.z, o4.z);
         o4.w = __fmaf_rn(a, u.w, o4.w);
       }
-      finish4(tid, top, total, o4);
+      finish(row, head0, vscale, tid, top, total, o4);
     }
-  } while (ps_next(piece, P.items, P.rows, units_of));
+  }
   if (gave_up) {  // copies still on their way end before the shared memory goes
     for (uint32_t i = filled > S::kStages ? filled - S::kStages : 0; i < filled; ++i)
       wait_full(&full_s[warp][i % S::kStages], (i / S::kStages) & 1, P.wait_ns);
