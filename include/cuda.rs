@@ -35,6 +35,7 @@ pub const MC_KV_BAD_ROW: c_int = 128;
 pub const MC_KV_WAIT: c_int = 256;
 pub const MC_TEST_SKIP_LOGIT_PUBLISH: c_int = 1;
 pub const MC_TEST_SKIP_BARRIER_ARRIVE: c_int = 2;
+pub const MC_TEST_SKIP_KV_ARRIVE: c_int = 4;
 
 /// mc_ctx: opaque (one device and stream; expert-parallel state).
 #[repr(C)]

@@ -376,7 +376,8 @@ int mc_rope_turns(float theta, float position_scale, int rot_dim, uint64_t* out)
  * slots[t] (NULL: slot t). Computed in fp32, rounded once where stored. The
  * *_stride are elements between tokens (multiples of 8), so q, k and v may be
  * parts of one fused projection row. q_out is q itself, with its stride, or
- * apart from q, k and v. Angles are exact modulo a turn at any position.
+ * apart from q, k and v; k and v lie outside the cache. Angles are exact modulo
+ * a turn at any position.
  * Every row of q_out is written, also those without a slot. Slots are
  * distinct; of two tokens with one slot either may stay, or parts of both. */
 int mc_qk_norm_rope(mc_ctx* ctx, const uint16_t* q, size_t q_stride, const uint16_t* k,
@@ -671,6 +672,9 @@ int mc_set_wait_limit(mc_ctx* ctx, unsigned long long ns);
 /* MC_TEST_SKIP_BARRIER_ARRIVE: the expert-parallel barrier of this rank
  * waits without arriving, so its wait runs out and sets status bit 8. */
 #define MC_TEST_SKIP_BARRIER_ARRIVE 2
+/* MC_TEST_SKIP_KV_ARRIVE: one warp of mc_paged_attention waits for copies that
+ * it does not report as arrived, so its wait runs out and sets MC_KV_WAIT. */
+#define MC_TEST_SKIP_KV_ARRIVE 4
 int mc_set_test_flags(mc_ctx* ctx, int flags);
 
 /* Evaluates the library's device math on x[n] into y[n]: op 0 = mc_exp,

@@ -316,6 +316,15 @@ extern "C" int mc_qk_norm_rope(mc_ctx* ctx, const uint16_t* q, size_t q_stride, 
     MC_REQUIRE(!overlap(q_out, out_bytes, k, 2 * (T * k_stride + kn)) &&
                    !overlap(q_out, out_bytes, v, 2 * (T * v_stride + kn)),
                "%s: q_out overlaps k or v", name);
+  const size_t row = kv_dtype == MC_DTYPE_BF16 ? 2 : 1;  // bytes of an element
+  const size_t cache_bytes =
+      row * (block_stride * (num_blocks - 1) + (size_t)n_kv_heads * block_size * head_dim);
+  const void* const rows[2] = {k, v};
+  const size_t strides[2] = {k_stride, v_stride};
+  for (int i = 0; i < 2; ++i)
+    MC_REQUIRE(!overlap(rows[i], 2 * (T * strides[i] + kn), k_cache, cache_bytes) &&
+                   !overlap(rows[i], 2 * (T * strides[i] + kn), v_cache, cache_bytes),
+               "%s: k or v lies in the cache", name);
   MC_REQUIRE(ctx, "%s: null context", name);
   McDeviceGuard dev(ctx->device);
   MC_CUDA(dev.error());

@@ -23,7 +23,7 @@ def lib():
     return _lib.lib()
 
 
-CACHE = dict(k_cache=0x10000, v_cache=0x20000, kv_dtype=_lib.DTYPE_BF16, num_blocks=8, block_size=16,
+CACHE = dict(k_cache=0x100000, v_cache=0x200000, kv_dtype=_lib.DTYPE_BF16, num_blocks=8, block_size=16,
              block_stride=8 * 16 * 64)
 # arguments in order; every pointer is a made-up aligned address that nothing reads
 CALLS = {
@@ -89,9 +89,12 @@ REFUSED = [
     ("mc_qk_norm_rope", dict(q_out=0x1000010), "overlaps q"),
     ("mc_qk_norm_rope", dict(q_out=0x2000000), "overlaps k or v"),
     ("mc_qk_norm_rope", dict(eps=INF), "eps"),
+    ("mc_qk_norm_rope", dict(k=0x100000), "in the cache"),
+    ("mc_qk_norm_rope", dict(v=0x200400), "in the cache"),
+    ("mc_qk_norm_rope", dict(n_tokens=(1 << 30) + 1), "n_tokens"),
     ("mc_qk_norm_rope", dict(block_stride=8 * 16 * 64 - 64), "block stride"),
     ("mc_qk_norm_rope", dict(block_stride=8 * 16 * 64 + 8), "multiple of head_dim"),
-    ("mc_qk_norm_rope", dict(k_cache=0x10008), "16-byte"),
+    ("mc_qk_norm_rope", dict(k_cache=0x100008), "16-byte"),
     ("mc_qk_norm_rope", dict(k_scale=0x100), "e4m3"),
     ("mc_paged_attention", dict(n_rows=-1), "n_rows"),
     ("mc_paged_attention", dict(n_heads=30), "query heads"),
