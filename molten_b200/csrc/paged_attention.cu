@@ -27,10 +27,13 @@
 // keys and up, 14% longer for e4m3 rows of 64 bytes, and 1.7 times as long for
 // pages of one key: a copy costs an SM some 47 cycles whatever its size.)
 //
-// Rounding of P. Eight heads fill rows 0-7 of the 16-row tile; P is split
-// into high and low parts (bf16 + bf16, or f16 + f16 for an e4m3 cache) and
-// the low part rides in rows 8-15 at no cost, so P enters the product with
-// 16 bits or more and the output's own rounding is the only one that counts.
+// Rounding of P. P is split into high and low parts (bf16 + bf16, or f16 + f16
+// for an e4m3 cache), so it enters the product with 16 bits or more and the
+// output's own rounding is the only one that counts. Eight heads fill rows 0-7
+// of the 16-row tile, and the low parts ride in rows 8-15 at no cost; where
+// more than 8 heads share a KV head a tile takes 16 and the low parts cost
+// products of their own (16 heads a KV head, 64 rows of 4000 to 8200 keys of
+// 128: 472 us by eights, 250 us by sixteens; e4m3 277 and 176 us).
 // With an e4m3 cache K and V become f16 exactly, and Q becomes f16 scaled by
 // a power of two a row (its largest value near 1), which loses nothing above
 // 2^-24 of that value.
@@ -53,12 +56,11 @@
 namespace {
 
 constexpr int kMaxCtas = 512;
-constexpr int kHeads = 8;               // query heads of an item
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// A piece's partial result in the workspace: o[8][D], m[8], l[8].
-constexpr size_t part_floats(int D) { return (size_t)kHeads * D + 2 * kHeads; }
+// A piece's partial result in the workspace: o[heads][D], m[heads], l[heads] (8 or 16 heads).
+constexpr size_t part_floats(int D, int heads) { return (size_t)heads * D + 2 * heads; }
 constexpr size_t kCounterBytes = kMaxCtas * sizeof(uint32_t);
 
 struct PaParams {
@@ -160,8 +162,9 @@ __device__ __forceinline__ void e4m3x4_to_f16(uint32_t v, uint32_t& lo, uint32_t
 // n ^ turn with turn = 2 (k / kPart), ^ 4 for an odd key if a row is whole
 // lines, so that the 8 chunks a quarter-warp reads at once (2 keys x 4 chunks
 // of K, 4 parts x 2 chunks of V) fall into different banks.
-template <int D, bool F8>
+template <int D, bool F8, int HEADS>
 struct Shape {
+  static constexpr int kHeads = HEADS;            // query heads of an item: 8 or 16
   static constexpr int kRow = D * (F8 ? 1 : 2);   // bytes of a key's row
   static constexpr int kChunks = kRow / 16;       // 16-byte chunks of a row
   static constexpr int kStep = kRow == 256 ? 16 : 32;  // keys a warp takes at once, one a lane
@@ -169,8 +172,8 @@ struct Shape {
   static constexpr int kHalf = kStep * kRow;      // K or V of a step
   static constexpr int kStage = 2 * kHalf;
   static constexpr int kWarps = 4;
-  static constexpr int kStages = kRow == 64 ? 4 : D == 64 ? 3 : 2;
-  static constexpr int kPerSm = kRow == 64 ? 3 : 2;  // CTAs an SM holds at once
+  static constexpr int kStages = kRow == 64 ? 4 : D == 64 && HEADS == 8 ? 3 : 2;
+  static constexpr int kPerSm = kRow == 64 && HEADS == 8 ? 3 : 2;  // CTAs an SM holds at once
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kUnit = kWarps * kStep;    // keys of a (small) unit
   static constexpr int kORow = D + 4;             // floats of a row in o
@@ -193,10 +196,11 @@ __device__ __forceinline__ int v_dim(int nt, int n) {
   return 64 * (nt / 8) + 8 * n + nt % 8;
 }
 
-template <int D, bool F8>
-__global__ void __launch_bounds__(Shape<D, F8>::kThreads, (Shape<D, F8>::kPerSm))
+template <int D, bool F8, int HEADS>
+__global__ void __launch_bounds__(Shape<D, F8, HEADS>::kThreads, (Shape<D, F8, HEADS>::kPerSm))
 paged_attention_kernel(const PaParams P) {
-  using S = Shape<D, F8>;
+  using S = Shape<D, F8, HEADS>;
+  constexpr int kHeads = HEADS, kM = HEADS / 8;  // kM: heads lane/4 and, of 16, 8 + lane/4
   constexpr int kT = D / 8;              // n-tiles of P.V
   constexpr int kZ = S::kStep / 16;
   constexpr uint32_t kAll = (1u << S::kPart) - 1;
@@ -374,15 +378,19 @@ paged_attention_kernel(const PaParams P) {
   // A piece's queries, as stored: row lane/4 of the tile (heads past the item's are zero), bf16
   // dims 8 (c + 4 i), e4m3 16 c + 64 (i / 2) + 8 (i % 2). They are asked for while the piece before
   // is merged, when its sums have left the registers.
-  uint4 q_raw[D / 32];
+  uint4 q_raw[kM][D / 32];
   auto load_q = [&](const PsCursor& p) {
-    const int kvh = p.item / P.subs, sub = p.item - kvh * P.subs, h = sub * kHeads + hr;
-    const uint4* q = reinterpret_cast<const uint4*>(P.q + (size_t)p.row * P.q_stride +
-                                                    (size_t)(kvh * P.group + h) * D);
+    const int kvh = p.item / P.subs, sub = p.item - kvh * P.subs;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      q_raw[i] = make_uint4(0, 0, 0, 0);
-      if (h < P.group) q_raw[i] = __ldg(q + (F8 ? 2 * c + 8 * (i / 2) + i % 2 : c + 4 * i));
+    for (int u = 0; u < kM; ++u) {
+      const int h = sub * kHeads + 8 * u + hr;
+      const uint4* q = reinterpret_cast<const uint4*>(P.q + (size_t)p.row * P.q_stride +
+                                                      (size_t)(kvh * P.group + h) * D);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        q_raw[u][i] = make_uint4(0, 0, 0, 0);
+        if (h < P.group) q_raw[u][i] = __ldg(q + (F8 ? 2 * c + 8 * (i / 2) + i % 2 : c + 4 * i));
+      }
     }
   };
   load_q(piece);
@@ -396,58 +404,65 @@ paged_attention_kernel(const PaParams P) {
     const float vscale = F8 && P.v_scale ? P.v_scale[kvh] : 1.0f;
 
     // ---- Q's fragments
-    uint32_t qa[D / 16][2];
-    float qk = P.scale_log2;
-    if (!F8) {
+    uint32_t qa[kM][D / 16][2];
+    float qk[kM];
 #pragma unroll
-      for (int i = 0; i < kKLoads; ++i) {
-        qa[2 * i][0] = q_raw[i].x;
-        qa[2 * i][1] = q_raw[i].y;
-        qa[2 * i + 1][0] = q_raw[i].z;
-        qa[2 * i + 1][1] = q_raw[i].w;
-      }
-    } else {
-      float f[D / 4];
-      float top = 0.0f;
+    for (int u = 0; u < kM; ++u) {
+      qk[u] = P.scale_log2;
+      if (!F8) {
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float2 p = unpack2<false>(word(q_raw[i], x));
-          f[8 * i + 2 * x] = p.x;
-          f[8 * i + 2 * x + 1] = p.y;
-          top = fmaxf(top, fmaxf(fabsf(p.x), fabsf(p.y)));
+        for (int i = 0; i < kKLoads; ++i) {
+          qa[u][2 * i][0] = q_raw[u][i].x;
+          qa[u][2 * i][1] = q_raw[u][i].y;
+          qa[u][2 * i + 1][0] = q_raw[u][i].z;
+          qa[u][2 * i + 1][1] = q_raw[u][i].w;
         }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^-e with 2^e <= top < 2^(e+1); 1 for zero, subnormal or infinite rows
-      const int e = (int)(__float_as_uint(top) >> 23) - 127;
-      const bool plain = e < -126 || e > 126;
-      const float down = plain ? 1.0f : __uint_as_float((uint32_t)(127 - e) << 23);
-      const float up = plain ? 1.0f : __uint_as_float((uint32_t)(127 + e) << 23);
+      } else {
+        float f[D / 4];
+        float top = 0.0f;
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i)
+        for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-          qa[i][x] = pack2<true>(f[4 * i + 2 * x] * down, f[4 * i + 2 * x + 1] * down);
-      qk *= up;
-      if (P.k_scale) qk *= P.k_scale[kvh];
+          for (int x = 0; x < 4; ++x) {
+            const float2 p = unpack2<false>(word(q_raw[u][i], x));
+            f[8 * i + 2 * x] = p.x;
+            f[8 * i + 2 * x + 1] = p.y;
+            top = fmaxf(top, fmaxf(fabsf(p.x), fabsf(p.y)));
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^-e with 2^e <= top < 2^(e+1); 1 for zero, subnormal or infinite rows
+        const int e = (int)(__float_as_uint(top) >> 23) - 127;
+        const bool plain = e < -126 || e > 126;
+        const float down = plain ? 1.0f : __uint_as_float((uint32_t)(127 - e) << 23);
+        const float up = plain ? 1.0f : __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            qa[u][i][x] = pack2<true>(f[4 * i + 2 * x] * down, f[4 * i + 2 * x + 1] * down);
+        qk[u] *= up;
+        if (P.k_scale) qk[u] *= P.k_scale[kvh];
+      }
+      // a factor above zero keeps the order of the scores (and -inf times it is -inf)
+      if (qk[u] < 0.0f) {
+        qk[u] = -qk[u];
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) qa[u][i][x] ^= 0x80008000u;
+      }
+      qk[u] = fmaxf(qk[u], 1e-37f);
     }
-    // a factor above zero keeps the order of the scores (and -inf times it is -inf)
-    if (qk < 0.0f) {
-      qk = -qk;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) qa[i][x] ^= 0x80008000u;
-    }
-    qk = fmaxf(qk, 1e-37f);
+
     float o[kT][4];
 #pragma unroll
     for (int i = 0; i < kT; ++i)
 #pragma unroll
       for (int x = 0; x < 4; ++x) o[i][x] = 0.0f;
-    float m = -INFINITY;
+    float m[kM];
+#pragma unroll
+    for (int u = 0; u < kM; ++u) m[u] = -INFINITY;
     float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // sums of P, a product with a column of ones
 
     for (int base = lo + warp * S::kStep; base < hi; base += S::kUnit) {
@@ -461,65 +476,98 @@ paged_attention_kernel(const PaParams P) {
       const uint8_t* k1 = k0 + k_flip;
       const uint8_t* v0 = ring + stage * S::kStage + S::kHalf + v_at;
       const uint8_t* v1 = v0 + v_flip;
-      // ---- scores for 8 heads; key kPart c + 4 z + 2 j + x in t[z][2 j + x]
-      float t[kZ][4];
+      // ---- scores; of key kPart c + 4 z + 2 j + x in t[u][z][2 j + x]
+      float t[kM][kZ][4];
 #pragma unroll
       for (int z = 0; z < kZ; ++z)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          auto a = [&](int u, int i, int x) { return u < kM ? qa[u % kM][i][x] : 0u; };
 #pragma unroll
           for (int i = 0; i < kKLoads; ++i) {
             const uint4 w = *reinterpret_cast<const uint4*>(
                 (i & 1 ? k1 : k0) + (4 * z + 2 * j) * S::kRow + 128 * (i >> 1));
             if (!F8) {
-              mma16816<false>(s, qa[2 * i][0], 0u, qa[2 * i][1], 0u, w.x, w.y);
-              mma16816<false>(s, qa[2 * i + 1][0], 0u, qa[2 * i + 1][1], 0u, w.z, w.w);
+              mma16816<false>(s, a(0, 2 * i, 0), a(1, 2 * i, 0), a(0, 2 * i, 1), a(1, 2 * i, 1), w.x,
+                              w.y);
+              mma16816<false>(s, a(0, 2 * i + 1, 0), a(1, 2 * i + 1, 0), a(0, 2 * i + 1, 1),
+                              a(1, 2 * i + 1, 1), w.z, w.w);
             } else {
 #pragma unroll
               for (int x = 0; x < 4; ++x) {
+                const int k = 4 * i + x;
                 uint32_t b0, b1;
                 e4m3x4_to_f16(word(w, x), b0, b1);
-                mma16816<true>(s, qa[4 * i + x][0], 0u, qa[4 * i + x][1], 0u, b0, b1);
+                mma16816<true>(s, a(0, k, 0), a(1, k, 0), a(0, k, 1), a(1, k, 1), b0, b1);
               }
             }
           }
-          t[z][2 * j] = s[0];
-          t[z][2 * j + 1] = s[1];
+#pragma unroll
+          for (int u = 0; u < kM; ++u) {
+            t[u][z][2 * j] = s[2 * u];
+            t[u][z][2 * j + 1] = s[2 * u + 1];
+          }
         }
-      // ---- running maximum and sum of head lane/4
+      // ---- running maxima
       if (live != kAll) {
 #pragma unroll
         for (int i = 0; i < 4 * kZ; ++i)
-          if (!(live >> i & 1u)) t[i / 4][i % 4] = -INFINITY;
+          if (!(live >> i & 1u)) {
+#pragma unroll
+            for (int u = 0; u < kM; ++u) t[u][i / 4][i % 4] = -INFINITY;
+          }
       }
-      float top = fmaxf(fmaxf(t[0][0], t[0][1]), fmaxf(t[0][2], t[0][3]));
+      float m_use[kM], m_new[kM];
+      bool grown = false;
 #pragma unroll
-      for (int z = 1; z < kZ; ++z)
-        top = fmaxf(top, fmaxf(fmaxf(t[z][0], t[z][1]), fmaxf(t[z][2], t[z][3])));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float m_new = fmaxf(m, top * qk);
-      const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-      if (__any_sync(0xffffffffu, m_new != m)) {
-        const float a = ex2(m - m_use);
+      for (int u = 0; u < kM; ++u) {
+        float top = fmaxf(fmaxf(t[u][0][0], t[u][0][1]), fmaxf(t[u][0][2], t[u][0][3]));
 #pragma unroll
-        for (int x = 0; x < 4; ++x) l4[x] *= a;
+        for (int z = 1; z < kZ; ++z)
+          top = fmaxf(top, fmaxf(fmaxf(t[u][z][0], t[u][z][1]), fmaxf(t[u][z][2], t[u][z][3])));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        m_new[u] = fmaxf(m[u], top * qk[u]);
+        m_use[u] = m_new[u] == -INFINITY ? 0.0f : m_new[u];
+        grown |= m_new[u] != m[u];
+      }
+      if (__any_sync(0xffffffffu, grown)) {
+        float a[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) a[u] = ex2(m[u % kM] - m_use[u % kM]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) l4[x] *= a[x / 2];
 #pragma unroll
         for (int i = 0; i < kT; ++i)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) o[i][x] *= a;
-        m = m_new;
+          for (int x = 0; x < 4; ++x) o[i][x] *= a[x / 2];
+#pragma unroll
+        for (int u = 0; u < kM; ++u) m[u] = m_new[u];
       }
 #pragma unroll
       for (int z = 0; z < kZ; ++z) {
-        float p[4];
+        // P's high and low parts
+        uint32_t high[kM][2], low[kM][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = ex2(__fmaf_rn(t[z][i], qk, -m_use));
-        const uint32_t h0 = pack2<F8>(p[0], p[1]), h1 = pack2<F8>(p[2], p[3]);
-        const float2 g0 = unpack2<F8>(h0), g1 = unpack2<F8>(h1);
-        const uint32_t w0 = pack2<F8>(p[0] - g0.x, p[1] - g0.y);
-        const uint32_t w1 = pack2<F8>(p[2] - g1.x, p[3] - g1.y);
+        for (int u = 0; u < kM; ++u)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float p0 = ex2(__fmaf_rn(t[u][z][2 * j], qk[u], -m_use[u]));
+            const float p1 = ex2(__fmaf_rn(t[u][z][2 * j + 1], qk[u], -m_use[u]));
+            high[u][j] = pack2<F8>(p0, p1);
+            const float2 g = unpack2<F8>(high[u][j]);
+            low[u][j] = pack2<F8>(p0 - g.x, p1 - g.y);
+          }
+        // 8 heads: the low parts are rows 8-15; 16 heads: a product of their own
+        auto weigh = [&](float* sum, uint32_t b0, uint32_t b1) {
+          if (kM == 1) {
+            mma16816<F8>(sum, high[0][0], low[0][0], high[0][1], low[0][1], b0, b1);
+          } else {
+            mma16816<F8>(sum, high[0][0], high[kM - 1][0], high[0][1], high[kM - 1][1], b0, b1);
+            mma16816<F8>(sum, low[0][0], low[kM - 1][0], low[0][1], low[kM - 1][1], b0, b1);
+          }
+        };
         uint32_t v[4][kVWords];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -547,15 +595,14 @@ paged_attention_kernel(const PaParams P) {
           }
         }
         constexpr uint32_t kOnes = F8 ? 0x3c003c00u : 0x3f803f80u;
-        mma16816<F8>(l4, h0, w0, h1, w1, kOnes, kOnes);
-        // ---- o += P V: rows 0-7 the high parts, rows 8-15 the low parts
+        weigh(l4, kOnes, kOnes);
+        // ---- o += P V
         if (!F8) {
 #pragma unroll
           for (int i = 0; i < kT / 2; ++i) {
-            mma16816<false>(o[2 * i], h0, w0, h1, w1, __byte_perm(v[0][i], v[1][i], 0x5410),
-                            __byte_perm(v[2][i], v[3][i], 0x5410));
-            mma16816<false>(o[2 * i + 1], h0, w0, h1, w1, __byte_perm(v[0][i], v[1][i], 0x7632),
-                            __byte_perm(v[2][i], v[3][i], 0x7632));
+            weigh(o[2 * i], __byte_perm(v[0][i], v[1][i], 0x5410), __byte_perm(v[2][i], v[3][i], 0x5410));
+            weigh(o[2 * i + 1], __byte_perm(v[0][i], v[1][i], 0x7632),
+                  __byte_perm(v[2][i], v[3][i], 0x7632));
           }
         } else {
 #pragma unroll
@@ -566,8 +613,7 @@ paged_attention_kernel(const PaParams P) {
             e4m3x4_to_f16(__byte_perm(v[2][i], v[3][i], 0x5140), b1[0], b1[1]);
             e4m3x4_to_f16(__byte_perm(v[2][i], v[3][i], 0x7362), b1[2], b1[3]);
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-              mma16816<true>(o[4 * i + x], h0, w0, h1, w1, b0[x], b1[x]);
+            for (int x = 0; x < 4; ++x) weigh(o[4 * i + x], b0[x], b1[x]);
           }
         }
       }
@@ -580,26 +626,36 @@ paged_attention_kernel(const PaParams P) {
     }
 
     // ---- the warps' results of this piece
-    float l = l4[0] + l4[2];
-    if (gave_up) l = __uint_as_float(0x7fc00000u);  // what did not arrive makes the result NaN
-    __syncthreads();  // the piece before is done with the shared arrays
-    if (c == 0) {
-      m_s[warp][hr] = m;
-      l_s[warp][hr] = l;
+    if (kM == 1) {  // the low parts' rows
+      l4[0] += l4[2];
+#pragma unroll
+      for (int i = 0; i < kT; ++i)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) o[i][x] += o[i][x + 2];
     }
+    if (gave_up) l4[0] = l4[2] = __uint_as_float(0x7fc00000u);  // what did not arrive: NaN
+    __syncthreads();  // the piece before is done with the shared arrays
 #pragma unroll
-    for (int i = 0; i < kT; i += 4)
+    for (int u = 0; u < kM; ++u) {
+      const int h = 8 * u + hr;
+      if (c == 0) {
+        m_s[warp][h] = m[u];
+        l_s[warp][h] = l4[2 * u];
+      }
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-        *reinterpret_cast<float4*>(o_s + (warp * kHeads + hr) * S::kORow + v_dim<D, F8>(i, 2 * c + x)) =
-            make_float4(o[i][x] + o[i][x + 2], o[i + 1][x] + o[i + 1][x + 2],
-                        o[i + 2][x] + o[i + 2][x + 2], o[i + 3][x] + o[i + 3][x + 2]);
+      for (int i = 0; i < kT; i += 4)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          *reinterpret_cast<float4*>(o_s + (warp * kHeads + h) * S::kORow + v_dim<D, F8>(i, 2 * c + x)) =
+              make_float4(o[i][2 * u + x], o[i + 1][2 * u + x], o[i + 2][2 * u + x],
+                          o[i + 3][2 * u + x]);
+    }
     const bool begins = piece.unit == 0, ends = piece.unit + piece.units == piece.n;
     const int n_units = piece.n, first_unit = u_end - piece.left - piece.unit;
     more_pieces = ps_next(piece, P.items, P.rows, units_of);
     if (more_pieces) load_q(piece);
     __syncthreads();
-    float* part = P.parts + part_floats(D) * (2 * (size_t)cta + (begins ? 1 : 0));
+    float* part = P.parts + part_floats(D, kHeads) * (2 * (size_t)cta + (begins ? 1 : 0));
     for (int at = tid; at < heads * D / 4; at += S::kThreads) {
       const int h = 4 * at / D, d = 4 * at % D;
       float mx = m_s[0][h];
@@ -643,12 +699,11 @@ paged_attention_kernel(const PaParams P) {
     __syncthreads();
     if (!last_s) continue;
     auto part_of = [&](int x) {
-      return P.parts + part_floats(D) * (2 * (size_t)x + (x == first_cta ? 1 : 0));
+      return P.parts + part_floats(D, kHeads) * (2 * (size_t)x + (x == first_cta ? 1 : 0));
     };
-    // Four elements a thread (or twice four), the pieces shared by `shares` threads for each, 12
+    // Four elements a thread (or kQ times four), the pieces shared by `shares` threads for each, 12
     // loads of them in flight; the shares' results meet in o_s, which is free here.
-    constexpr int kQ = kHeads * D / 4 > S::kThreads ? 2 : 1, kB = 12 / kQ;
-    static_assert(kQ * S::kThreads >= kHeads * D / 4, "a thread for each quad");
+    constexpr int kQ = (kHeads * D / 4 + S::kThreads - 1) / S::kThreads, kB = 12 / kQ;
     const int quads = heads * D / 4, shares = S::kThreads > quads ? S::kThreads / quads : 1;
     const int share = tid / quads, at0 = shares > 1 ? tid % quads : tid;
     float mx[kQ], sum[kQ];
@@ -734,14 +789,16 @@ paged_attention_kernel(const PaParams P) {
   if (gave_up) mc_cp_async_wait_all();
 }
 
-template <int D, bool F8>
-int launch_attention(mc_ctx* ctx, PaParams& P) {
-  using S = Shape<D, F8>;
+template <int D, bool F8, int HEADS>
+int launch_heads(mc_ctx* ctx, PaParams& P) {
+  using S = Shape<D, F8, HEADS>;
+  P.subs = (P.group + HEADS - 1) / HEADS;
+  P.items = P.K * P.subs;
   const long long items = (long long)P.rows * P.items;
   P.small_unit = ps_small_unit(S::kUnit, items, P.capacity);
   if (P.small_unit == 0)
     return mc_fail(MC_EUNSUPPORTED, "paged_attention: %lld row and head groups", items);
-  auto fn = paged_attention_kernel<D, F8>;
+  auto fn = paged_attention_kernel<D, F8, HEADS>;
   MC_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
   long long g = (long long)ctx->num_sms * S::kPerSm;
   const long long most = ((long long)P.capacity + S::kUnit - 1) / S::kUnit * items;
@@ -751,11 +808,17 @@ int launch_attention(mc_ctx* ctx, PaParams& P) {
   return mc_after_launch("paged_attention_kernel");
 }
 
+// Items of 8 heads, or of 16 where more share a KV head (see the rounding of P above).
+template <int D, bool F8>
+int launch_attention(mc_ctx* ctx, PaParams& P) {
+  return P.group > 8 ? launch_heads<D, F8, 16>(ctx, P) : launch_heads<D, F8, 8>(ctx, P);
+}
+
 }  // namespace
 
 extern "C" size_t mc_paged_attention_workspace_bytes(int head_dim) {
   if (head_dim != 64 && head_dim != 128) return 0;
-  return kCounterBytes + 2 * (size_t)kMaxCtas * part_floats(head_dim) * sizeof(float);
+  return kCounterBytes + 2 * (size_t)kMaxCtas * part_floats(head_dim, 16) * sizeof(float);
 }
 
 extern "C" int mc_paged_attention(mc_ctx* ctx, const uint16_t* q, size_t q_stride, int n_rows,
@@ -798,9 +861,8 @@ extern "C" int mc_paged_attention(mc_ctx* ctx, const uint16_t* q, size_t q_strid
   MC_REQUIRE(ctx, "%s: null context", name);
   McDeviceGuard dev(ctx->device);
   MC_CUDA(dev.error());
-  const int group = n_heads / n_kv_heads, subs = (group + kHeads - 1) / kHeads;
   const long long capacity = (long long)table_width * block_size;
-  PaParams P{q, q_stride, n_rows, n_heads, n_kv_heads, group, subs, n_kv_heads * subs,
+  PaParams P{q, q_stride, n_rows, n_heads, n_kv_heads, n_heads / n_kv_heads, 0, 0,
                    k_cache, v_cache, num_blocks, block_size, (uint32_t)(block_stride / head_dim),
                    ps_div_of(block_size), k_scale, v_scale, block_table, n_req, table_width,
              (int)(capacity < 0x7fff0000ll ? capacity : 0x7fff0000ll), 0, kv_lens, row_req, window, scale * kLog2e,

@@ -1,7 +1,7 @@
 // How a paged-attention launch splits its work over CTAs: host/device
 // arithmetic only, so that the CPU tests run the same code.
 //
-// A work item is one query row and one group of up to 8 query heads that
+// A work item is one query row and one group of up to 8 or 16 query heads that
 // share a KV head. Its keys are cut into units of `unit` tokens (an item has
 // at least one, so that a row without keys is still written). The units of
 // all items in order -- row by row, within a row item by item -- are dealt

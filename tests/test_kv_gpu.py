@@ -321,7 +321,9 @@ EDGES = [0, 1, 2, 15, 16, 17, 31, 63, 64, 65, 127, 128, 129, 200]
     ([0], 4, 1, 64, 16, False, 0), ([1], 4, 1, 64, 16, True, 0), ([0, 0, 0], 4, 4, 128, 16, False, 0),
     ([5000, 0, 1, 12345, 64], 8, 2, 64, 16, False, 0), ([5000, 0, 1, 9001, 64], 8, 2, 128, 24, True, 0),
     ([40000], 2, 1, 64, 128, False, 0), ([40000], 3, 1, 128, 16, True, 0), ([40000, 300], 4, 2, 64, 16, False, 30001),
-    ([3] * 700, 4, 1, 64, 4, False, 0), (list(range(300)), 4, 2, 64, 16, False, 17)])
+    (EDGES, 16, 1, 64, 16, False, 0), (EDGES, 32, 2, 128, 16, True, 0), (EDGES, 24, 1, 128, 16, False, 33),
+    ([5000, 0, 1, 9001, 64], 48, 2, 64, 16, False, 0), ([5000, 0, 1, 9001, 64], 20, 2, 128, 16, True, 0),
+    ([20000], 16, 1, 128, 16, False, 0), ([20000, 7], 31, 1, 64, 16, True, 0), ([3] * 700, 4, 1, 64, 4, False, 0), (list(range(300)), 4, 2, 64, 16, False, 17)])
 def test_attention(cuda_ctx, lens, H, K, D, bs, fp8, window):
     q, cache, table, keys = attention_case(len(lens) + H + D + bs, lens, H, K, D, bs, fp8)
     out = torch.full_like(q, NAN)
