@@ -349,6 +349,7 @@ paged_attention_kernel(const PaParams P) {
   enter();
   seek();
   for (int i = 0; i < S::kStages && more; ++i) issue();
+  __syncwarp();  // live_s of the first steps
 
   int stage = 0;
   uint32_t phase = 0;

@@ -32,8 +32,9 @@ def ensure(cond: bool, msg: str) -> None:
 def _p(t: torch.Tensor | None) -> int | None:
     if t is None:
         return None
-    ensure(t.is_cuda, "tensors must be on the GPU")
-    ensure(t.is_contiguous(), "tensors must be contiguous")
+    if not (t.is_cuda and t.is_contiguous()):
+        ensure(t.is_cuda, "tensors must be on the GPU")
+        ensure(t.is_contiguous(), "tensors must be contiguous")
     return t.data_ptr()
 
 
@@ -122,14 +123,14 @@ class Context:
 
 def _bf16(*ts):
     for t in ts:
-        if t is not None:
-            ensure(t.dtype == torch.bfloat16, "expects BF16")
+        if t is not None and t.dtype is not torch.bfloat16:
+            ensure(False, "expects BF16")
 
 
 def _u32(*ts):
     for t in ts:
-        if t is not None:
-            ensure(t.dtype == torch.int32, "expects U32 (int32 storage)")
+        if t is not None and t.dtype is not torch.int32:
+            ensure(False, "expects U32 (int32 storage)")
 
 
 def copy_async(ctx: Context, dst: torch.Tensor, src: torch.Tensor) -> None:
