@@ -532,6 +532,7 @@ struct KvCache {
     ensure(k.shape.size() == 4 && v.shape == k.shape && v.dtype == k.dtype &&
                (k.dtype == DType::BF16 || k.dtype == DType::E4M3),
            "KV cache: k and v are alike, BF16 or E4M3 [blocks][KV heads][block size][head dim]");
+    ensure(k.numel() > 0, "KV cache: empty");
     for (const Tensor* s : {k_scale, v_scale})
       ensure(!s || (s->dtype == DType::F32 && s->numel() == k.dim(1)), "KV cache scales");
   }
@@ -607,8 +608,8 @@ inline void qk_norm_rope(Context& ctx, const Tensor& q, size_t q_stride, const T
   ensure(D == cache.head_dim() && k.shape == std::vector<int64_t>{T, K, D} &&
              k.dtype == DType::BF16 && (!v || (v->shape == k.shape && v->dtype == DType::BF16)),
          "qk_norm_rope k rows match the cache");
-  ensure((!q_norm_w || q_norm_w->numel() == D) && (!k_norm_w || k_norm_w->numel() == D),
-         "qk_norm_rope gains");
+  for (const Tensor* w : {q_norm_w, k_norm_w})
+    ensure(!w || (w->dtype == DType::BF16 && w->numel() == D), "qk_norm_rope gains");
   ensure(!turns || (turns->dtype == DType::U64 && positions), "qk_norm_rope turns");
   if (positions) i32(*positions, T, "positions");
   ensure(!slots || (slots->dtype == DType::U64 && slots->numel() == T), "qk_norm_rope slots");
@@ -704,7 +705,11 @@ inline void logits_process(Context& ctx, const Tensor& logits, const Tensor& out
 
 // Counts the drawn tokens in the rules' seen bitmap and counts.
 inline void logits_mark(Context& ctx, const Tensor& tokens, const LogitsRules& r, int vocab) {
+  const int64_t B = tokens.numel(), W = ((int64_t)vocab + 31) / 32;
   ensure(tokens.dtype == DType::U32, "drawn tokens");
+  ensure(!r.seen || (r.seen->dtype == DType::U32 && r.seen->numel() == B * W), "seen shape");
+  ensure(!r.counts || (r.counts->dtype == DType::U16 && r.counts->numel() == B * vocab),
+         "counts shape");
   check(mc_logits_mark(ctx.handle(), tokens.as<const uint32_t>(), (int)tokens.numel(),
                        maybe<uint32_t>(r.seen), maybe<uint16_t>(r.counts), vocab));
 }

@@ -376,7 +376,7 @@ int mc_rope_turns(float theta, float position_scale, int rot_dim, uint64_t* out)
  * slots[t] (NULL: slot t). Computed in fp32, rounded once where stored. The
  * *_stride are elements between tokens (multiples of 8), so q, k and v may be
  * parts of one fused projection row. q_out is q itself, with its stride, or
- * apart from q, k and v; k and v lie outside the cache. Angles are exact modulo
+ * apart from q, k and v; all four lie outside the cache. Angles are exact modulo
  * a turn at any position.
  * Every row of q_out is written, also those without a slot. Slots are
  * distinct; of two tokens with one slot either may stay, or parts of both. */

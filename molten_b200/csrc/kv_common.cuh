@@ -60,9 +60,11 @@ static inline int mc_check_kv_cache(const char* name, const void* k, const void*
              "%s: block stride %zu below a page of %zu elements", name, block_stride, page);
   MC_REQUIRE(block_stride % (size_t)head_dim == 0,
              "%s: block stride %zu not a multiple of head_dim", name, block_stride);
-  // rows are numbered in 32 bits (the memory of a GPU holds fewer of 64 bytes)
-  MC_REQUIRE(page / head_dim < 0xffffffffull &&
-                 block_stride / head_dim * (num_blocks - 1) + page / head_dim < 0xffffffffull,
+  // rows are numbered in 32 bits (the memory of a GPU holds fewer of 64 bytes); the stride by
+  // itself first, so that its product stays in 64
+  const size_t most = 0xffffffffull, step = num_blocks > 1 ? block_stride / head_dim : 0;
+  MC_REQUIRE(page / head_dim < most && step < most &&
+                 step * (num_blocks - 1) + page / head_dim < most,
              "%s: a cache of more than 2^32 - 2 rows", name);
   MC_REQUIRE(dtype == MC_DTYPE_E4M3 || (!k_scale && !v_scale),
              "%s: scales belong to an e4m3 cache", name);

@@ -12,10 +12,9 @@
 // running sums). A request is admitted whole or not at all.
 //
 // The work is a few hundred bytes to a few hundred KB, bound by latency: one
-// CTA (of as who threads as there are requests or rows to map where that
-// bounds the pages too, else the most), with what the maps need in shared
-// memory; above kMapsInPlan rows the maps (20 bytes a
-// token) go to a second, chained launch. The first launch writes the map
+// CTA (of as many threads as there are requests or rows to map, up to the
+// most), with what the maps need in shared memory; above kMapsInPlan rows the
+// maps (20 bytes a token) go to a second, chained launch. The first launch writes the map
 // entries of each request's first token; their position and kv_len tell the
 // second launch the request's old length and whether it was admitted, so
 // `seq_lens` may be `lens` itself.
@@ -313,7 +312,7 @@ __global__ void __launch_bounds__(kThreads) release_kernel(const ReleaseParams P
   }
 }
 
-// Above this who token rows the maps go to a launch of their own.
+// Above this many token rows the maps go to a launch of their own.
 constexpr int kMapsInPlan = 2048;
 
 // A thread for each request and row, whole warps.

@@ -14,9 +14,9 @@
 // every rule on, instructions, some 40 a token and lane. A thread takes 8
 // tokens: one 16-byte load of bf16 logits, one of counts, one byte of each
 // bitmap, the next span's on their way while it works on one (48 rows of
-// 128000 with all rules, in L2: 24 us without, 15 us). A CTA takes up to 4 spans of 2048 tokens of one row, so that a large
-// batch is one wave. Biases are a short sorted
-// list a row; each CTA looks through the part that can fall into its tokens
+// 128000 with all rules, in L2: 24 us without, 15 us). A CTA takes up to 4
+// spans of 2048 tokens of one row, so that a large batch is one wave. Biases
+// are a short sorted list a row; each CTA looks through the part that can fall into its tokens
 // (256 probes narrow a long list) and the thread at the first of a run of
 // equal ids adds the run up into shared memory, so no order of atomics enters.
 #include "kv_common.cuh"
@@ -364,7 +364,8 @@ extern "C" int mc_logits_process(mc_ctx* ctx, const void* logits, size_t logits_
                    (!counts || ((uintptr_t)counts / 2 % lane == la && mc_aligned(counts, 2) &&
                                 (batch == 1 || (size_t)vocab % lane == logits_stride % lane)));
   // CTAs a row: as many as one wave leaves it, in runs of at most kSpans spans
-  const int all = (vocab + (vec ? (int)lane - 1 : 0) + kSpan - 1) / kSpan, share = kResident * ctx->num_sms / batch;
+  const int all = (vocab + (vec ? (int)lane - 1 : 0) + kSpan - 1) / kSpan;
+  const int share = kResident * ctx->num_sms / batch;
   int spans = share > 0 ? (all + share - 1) / share : kSpans;
   spans = spans < 1 ? 1 : spans > kSpans ? kSpans : spans;
   P.spans = spans;
@@ -383,6 +384,8 @@ extern "C" int mc_logits_mark(mc_ctx* ctx, const uint32_t* tokens, int batch, ui
   MC_REQUIRE(vocab >= 1, "logits_mark: vocab %d", vocab);
   if (batch == 0) return MC_OK;
   MC_REQUIRE(tokens && (seen || counts), "logits_mark: null pointer");
+  MC_REQUIRE(mc_aligned(tokens, 4) && mc_aligned(seen, 4) && mc_aligned(counts, 2),
+             "logits_mark: misaligned tokens, seen or counts");
   MC_REQUIRE(ctx, "logits_mark: null context");
   McDeviceGuard dev(ctx->device);
   MC_CUDA(dev.error());

@@ -239,8 +239,9 @@ int launch_rope(mc_ctx* ctx, RopeParams& P) {
   const int most = kMaxThreads / (D / 8), parts = (P.rows + most - 1) / most;
   P.group = (P.rows + parts - 1) / parts;
   const int threads = (P.group * (D / 8) + 31) / 32 * 32;
-  // one wave: equal shares of the tokens for every CTA that fits, in equal batches
-  const int slots = kResident * ctx->num_sms / parts;
+  // one wave: equal shares of the tokens for every CTA that fits (at least one, where the parts
+  // alone are more than a wave), in equal batches
+  const int wave = kResident * ctx->num_sms, slots = wave > parts ? wave / parts : 1;
   P.share = (P.tokens + slots - 1) / slots;
   const int batches = (P.share + kBatch - 1) / kBatch;
   P.batch = (P.share + batches - 1) / batches;
@@ -253,6 +254,18 @@ int launch_rope(mc_ctx* ctx, RopeParams& P) {
 bool overlap(const void* p, size_t bytes, const void* q, size_t more) {
   const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
   return p && q && a < b + more && b < a + bytes;
+}
+
+// Of `tokens` rows of `an` bytes at a and of `bn` bytes at b, one each `a_step` / `b_step` bytes,
+// some share a byte. Rows of one step may interleave (parts of one fused row); of two steps,
+// their whole ranges count.
+bool rows_overlap(const void* a, size_t an, size_t a_step, const void* b, size_t bn, size_t b_step,
+                  size_t tokens) {
+  if (!overlap(a, (tokens - 1) * a_step + an, b, (tokens - 1) * b_step + bn)) return false;
+  if (tokens == 1 || a_step != b_step || a_step == 0) return true;
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  const size_t behind = y >= x ? (y - x) % a_step : (a_step - (x - y) % a_step) % a_step;
+  return behind < an || behind + bn > a_step;
 }
 
 }  // namespace
@@ -305,26 +318,26 @@ extern "C" int mc_qk_norm_rope(mc_ctx* ctx, const uint16_t* q, size_t q_stride, 
   MC_REQUIRE(q_stride <= far && k_stride <= far && v_stride <= far && q_out_stride <= far,
              "%s: token stride out of range", name);
   MC_REQUIRE(n_tokens <= 1 || q_out_stride >= qn, "%s: q_out rows overlap", name);
-  const size_t T = (size_t)n_tokens - 1;
-  const size_t q_bytes = 2 * (T * q_stride + qn), out_bytes = 2 * (T * q_out_stride + qn);
+  const size_t T = (size_t)n_tokens, q_step = 2 * q_stride, out_step = 2 * q_out_stride;
   // q_out may be q itself (a lane writes the 16 bytes it read), nothing else that is read
-  MC_REQUIRE((q_out == q && (q_out_stride == q_stride || n_tokens == 1)) ||
-                 !overlap(q_out, out_bytes, q, q_bytes),
+  MC_REQUIRE((q_out == q && (q_out_stride == q_stride || T == 1)) ||
+                 !rows_overlap(q_out, 2 * qn, out_step, q, 2 * qn, q_step, T),
              "%s: q_out overlaps q without being q", name);
-  // parts of one fused row interleave: only a contiguous q_out can be judged against k and v
-  if (q_out != q)
-    MC_REQUIRE(!overlap(q_out, out_bytes, k, 2 * (T * k_stride + kn)) &&
-                   !overlap(q_out, out_bytes, v, 2 * (T * v_stride + kn)),
-               "%s: q_out overlaps k or v", name);
-  const size_t row = kv_dtype == MC_DTYPE_BF16 ? 2 : 1;  // bytes of an element
-  const size_t cache_bytes =
-      row * (block_stride * (num_blocks - 1) + (size_t)n_kv_heads * block_size * head_dim);
-  const void* const rows[2] = {k, v};
-  const size_t strides[2] = {k_stride, v_stride};
-  for (int i = 0; i < 2; ++i)
-    MC_REQUIRE(!overlap(rows[i], 2 * (T * strides[i] + kn), k_cache, cache_bytes) &&
-                   !overlap(rows[i], 2 * (T * strides[i] + kn), v_cache, cache_bytes),
-               "%s: k or v lies in the cache", name);
+  MC_REQUIRE(!rows_overlap(q_out, 2 * qn, out_step, k, 2 * kn, 2 * k_stride, T) &&
+                 !rows_overlap(q_out, 2 * qn, out_step, v, 2 * kn, 2 * v_stride, T),
+             "%s: q_out overlaps k or v", name);
+  const size_t size = kv_dtype == MC_DTYPE_BF16 ? 2 : 1;  // bytes of an element
+  const size_t cache_bytes = size * (block_stride * ((size_t)num_blocks - 1) +
+                                     (size_t)n_kv_heads * block_size * head_dim);
+  const void* const rows[4] = {q, k, v, q_out};
+  const size_t bytes[4] = {2 * qn, 2 * kn, 2 * kn, 2 * qn};
+  const size_t steps[4] = {q_step, 2 * k_stride, 2 * v_stride, out_step};
+  for (int i = 0; i < 4; ++i) {
+    const size_t n = (T - 1) * steps[i] + bytes[i];
+    MC_REQUIRE(!overlap(rows[i], n, k_cache, cache_bytes) &&
+                   !overlap(rows[i], n, v_cache, cache_bytes),
+               "%s: q, k, v or q_out lies in the cache", name);
+  }
   MC_REQUIRE(ctx, "%s: null context", name);
   McDeviceGuard dev(ctx->device);
   MC_CUDA(dev.error());

@@ -66,19 +66,22 @@ def _rows(ctx: Context, t: torch.Tensor, shape: torch.Size, what: str) -> tuple[
         ensure(_on(ctx, t), f"{what} must be on {ctx.device}")
         ensure(False, f"{what} shape")
     token, head, one = t.stride()
+    if shape[0] <= 1:
+        token = shape[1] * shape[2]  # a single row's distance to the next says nothing
     if one != 1 or head != shape[2]:
         ensure((one == 1 or shape[2] == 1) and (head == shape[2] or shape[1] == 1),
                f"{what}: a row's heads must be contiguous")
     return t.data_ptr(), token
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class KvCache:
     """Pages of K and V: [num_blocks, KV heads, block_size, head_dim] in bf16
     or float8_e4m3fn, contiguous but for the distance between pages (the same
     for both, so K and V may be the halves of one [num_blocks, 2, ...]
     tensor); ``k_scale`` / ``v_scale``: optional f32 [KV heads] of an 8-bit
-    cache (stored = value / scale)."""
+    cache (stored = value / scale). The tensors stay the same ones: their
+    addresses are taken here."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor | None = None
@@ -90,6 +93,7 @@ class KvCache:
                "KV cache: k and v are alike, [blocks, KV heads, block size, head dim]")
         ensure(k.dtype in (torch.bfloat16, torch.float8_e4m3fn), "KV cache: BF16 or float8_e4m3fn")
         _, heads, size, dim = k.shape
+        ensure(k.numel() > 0, "KV cache: empty")
         for t in (k, v):
             ensure(t[0].is_contiguous() and (t.shape[0] == 1 or t.stride(0) == k.stride(0)),
                    "KV cache: pages must be contiguous, K's and V's equally far apart")
@@ -99,10 +103,10 @@ class KvCache:
         dt = _lib.DTYPE_BF16 if k.dtype == torch.bfloat16 else _lib.DTYPE_E4M3
         p = lambda s: None if s is None else s.data_ptr()  # noqa: E731
         stride = k.stride(0) if k.shape[0] > 1 else heads * size * dim
-        self.n_kv_heads, self.head_dim = heads, dim
-        self._index = k.get_device()
-        self._where = (k.data_ptr(), v.data_ptr(), dt, k.shape[0], size, stride)
-        self._scales = (p(self.k_scale), p(self.v_scale))
+        self.__dict__.update(
+            n_kv_heads=heads, head_dim=dim, _index=k.get_device(),
+            _where=(k.data_ptr(), v.data_ptr(), dt, k.shape[0], size, stride),
+            _scales=(p(self.k_scale), p(self.v_scale)))
 
     @property
     def block_size(self) -> int:
@@ -167,6 +171,7 @@ def rope_turns(rot_dim: int, theta: float = 1e6, position_scale: float = 1.0) ->
     """The rotation frequencies position_scale * theta^(-2i / rot_dim) as
     fractions of a turn per position in 64-bit fixed point: int64 [rot_dim / 2]
     on the host, to be uploaded once."""
+    ensure(rot_dim >= 2, f"rope_turns: rot_dim {rot_dim}")
     out = torch.empty(rot_dim // 2, dtype=torch.int64)
     _lib.call("mc_rope_turns", theta, position_scale, rot_dim, out.data_ptr())
     return out
@@ -254,20 +259,23 @@ class PagedBatch:
         i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device=dev)  # noqa: E731
         T = n_req if max_tokens is None else max_tokens
         self.ctx, self.block_size = ctx, block_size
-        self.lens, self.n_free = i32(n_req), i32(1)
-        self.block_table = torch.full((n_req, table_width), -1, dtype=torch.int32, device=dev)
-        self.free_list = torch.arange(num_blocks - 1, -1, -1, dtype=torch.int32, device=dev)
-        self.row_start, self.status = i32(n_req + 1), i32(1)
-        self.positions, self.token_req, self.kv_lens = i32(T), i32(T), i32(T)
-        self.slots = torch.zeros(T, dtype=torch.int64, device=dev)
+        with torch.cuda.stream(ctx.stream):
+            self.lens, self.n_free = i32(n_req), i32(1)
+            self.block_table = torch.full((n_req, table_width), -1, dtype=torch.int32, device=dev)
+            self.free_list = i32(num_blocks)
+            self.row_start, self.status = i32(n_req + 1), i32(1)
+            self.positions, self.token_req, self.kv_lens = i32(T), i32(T), i32(T)
+            self.slots = torch.zeros(T, dtype=torch.int64, device=dev)
         self.clear()
 
     def clear(self) -> None:
-        """Every request empty, every page free."""
-        self.lens.zero_()
-        self.status.zero_()
-        self.n_free.fill_(self.free_list.numel())
-        self.free_list.copy_(torch.arange(self.free_list.numel() - 1, -1, -1, dtype=torch.int32))
+        """Every request empty, every page free (on the context's stream, as all calls)."""
+        n = self.free_list.numel()
+        with torch.cuda.stream(self.ctx.stream):
+            self.lens.zero_()
+            self.status.zero_()
+            self.n_free.fill_(n)
+            torch.arange(n - 1, -1, -1, out=self.free_list)
 
     def plan(self, new_lens: torch.Tensor | None = None) -> None:
         """The next step: new_lens tokens (None: one each) for the requests."""
@@ -283,4 +291,5 @@ class PagedBatch:
     def check(self) -> None:
         """Waits for the stream and raises McError if a request was refused or
         an index was out of range since the last clear()."""
-        raise_on_status(self.status, "paged batch")
+        with torch.cuda.stream(self.ctx.stream):
+            raise_on_status(self.status, "paged batch")

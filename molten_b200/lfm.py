@@ -86,6 +86,11 @@ class Context:
             self._stream = s
         return self.h
 
+    @property
+    def stream(self) -> torch.cuda.Stream:
+        """The stream the context enqueues on: its own, or else the current one."""
+        return self._fixed_stream or torch.cuda.current_stream(self.device)
+
     def commit_wait(self) -> None:
         _lib.check(_lib.lib().mc_sync(self.h))
 

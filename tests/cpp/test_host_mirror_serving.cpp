@@ -83,6 +83,17 @@ int main() {
     kernels::paged_attention(ctx, q, bad, table, map, nullptr, 0, 0.125f, out, &lse, ws);
   });
 
+  bad = cache;
+  bad.k = bad.v = T({8, 0, 16, 64}, DType::BF16);
+  expect_error("empty cache", "empty", [&] {
+    kernels::paged_attention(ctx, q, bad, table, map, nullptr, 0, 0.125f, out, &lse, ws);
+  });
+  const Tensor wide = T({64}, DType::F32);
+  expect_error("gains of another type", "gains", [&] {
+    kernels::qk_norm_rope(ctx, q, 0, k, 0, &v, 0, &wide, &gain, 1e-5f, &map, &turns, false, out, 0,
+                          cache, &slots);
+  });
+
   const Tensor logits = T({2, 1000}, DType::BF16), to = T({2, 1000}, DType::BF16);
   const Tensor seen = T({2, 32}, DType::U32), counts = T({2, 1000}, DType::U16);
   const Tensor f = T({2}, DType::F32), best = T({2}, DType::U64), toks = T({2}, DType::U32);
@@ -95,6 +106,8 @@ int main() {
                [&] { kernels::logits_process(ctx, logits, to, r, &best); });
   expect_error("mark reaches the ABI", "null context",
                [&] { kernels::logits_mark(ctx, toks, r, 1000); });
+  expect_error("mark of another vocabulary", "seen shape",
+               [&] { kernels::logits_mark(ctx, toks, r, 2000); });
   r.seen = &counts;
   expect_error("rules seen", "seen shape", [&] { kernels::logits_process(ctx, logits, to, r); });
   r.seen = nullptr;

@@ -212,6 +212,35 @@ def test_norm_rope_and_store(cuda_ctx, T, H, K, D, rot, inter, fp8, far):
     assert st.item() == 0 and torch.equal(q, q0) and torch.equal(k, k0)
 
 
+@pytest.mark.parametrize("H", [7000, 8000, 16384])
+def test_norm_rope_more_heads_than_a_wave(cuda_ctx, H):
+    """Above 24 heads of 128 for each of a wave's CTAs (7104 and more on 148 SMs) one row of CTAs takes every token."""
+    T, K, D = 3, 1, 128
+    g, q, k, v, qw, kw, c = rope_case(H, T, H, K, D, False, bs=4, fused=False)
+    pos, slots = i32([5, 0, 70000]), torch.tensor([2, 0, 1], device="cuda")
+    out = torch.empty(T, H, D, dtype=torch.bfloat16, device="cuda")
+    kv.qk_norm_rope(cuda_ctx, q, k, v, qw, kw, pos, kv.rope_turns(D).cuda(), out, c, slots)
+    want, size = ref.norm_rope(q, qw, pos, [1e6 ** (-2 * i / D) for i in range(D // 2)], D, False, 1e-5)
+    assert bool(((out.double() - want).abs() <= ref.BF16_HALF * want.abs() + 1.01 * ref.norm_rope_error(D) * size).all())
+    check_store(c.v, [2, 0, 1], v.double(), torch.zeros_like(v, dtype=torch.float64), None, 4, 0x35)
+
+
+def test_norm_rope_in_place_in_a_fused_row_and_of_one_token(cuda_ctx):
+    for T in (5, 1):
+        g, q, k, v, qw, kw, c = rope_case(9, T, 4, 2, 64, False, bs=4)
+        pos = torch.arange(T, device="cuda", dtype=I32) + 9
+        turns = kv.rope_turns(64).cuda()
+        out = torch.empty(T, 4, 64, dtype=torch.bfloat16, device="cuda")
+        kv.qk_norm_rope(cuda_ctx, q, k, v, qw, kw, pos, turns, out, c)
+        first = c.k.clone()
+        k0 = k.clone()
+        if T == 1:  # a row whose stride to the next, which is not there, is odd
+            q = q.as_strided(q.shape, (q.stride(0) + 1, 64, 1))
+        kv.qk_norm_rope(cuda_ctx, q, k, v, qw, kw, pos, turns, q, c)
+        assert torch.equal(q, out) and torch.equal(k, k0)
+        assert torch.equal(c.k.view(torch.uint8), first.view(torch.uint8))
+
+
 def test_norm_rope_in_place_without_v_norm_or_slots(cuda_ctx):
     T, H, K, D = 6, 4, 2, 64
     g, q, k, v, qw, kw, c = rope_case(1, T, H, K, D, False, blocks=1, bs=8, fused=False)
@@ -529,6 +558,27 @@ def test_offsets_past_32_bits(cuda_ctx):
 
 
 # ------------------------------------------------------------------ together
+
+def test_a_batch_on_the_stream_of_its_context():
+    """The bookkeeping's own tensors are made, cleared and read on the context's stream, whatever stream is current."""
+    from molten_b200 import lfm
+    ctx = lfm.Context(0, torch.cuda.Stream())
+    try:
+        for _ in range(20):
+            batch = kv.PagedBatch(ctx, 3, 6, 4, 2)
+            batch.plan()
+            batch.check()
+            assert batch.lens.tolist() == [1, 1, 1] and batch.slots.tolist() == [0, 4, 8]
+            batch.clear()
+            batch.plan()
+            batch.check()
+            assert batch.lens.tolist() == [1, 1, 1] and batch.block_table[:, 0].tolist() == [0, 1, 2]
+            batch.plan(i32([8, 0, 0]))  # outgrows its table
+            with pytest.raises(_lib.McError, match="outgrew"):
+                batch.check()
+    finally:
+        ctx.close()
+
 
 @pytest.mark.parametrize("fp8,captured", [(False, False), (True, False), (False, True)])
 def test_a_served_batch(cuda_ctx, fp8, captured):

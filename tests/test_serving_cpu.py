@@ -128,6 +128,19 @@ REFUSED = [
     ("mc_logits_process", dict(out_stride=500), "overlap"),
     ("mc_logits_mark", dict(seen=None, counts=None), "null"),
     ("mc_logits_mark", dict(batch=-1), "batch"),
+    # rows of one stride interleave (parts of a fused row) but share no byte
+    ("mc_qk_norm_rope", dict(q_out=0x1000000, k=0x1000010, k_stride=2048), "overlaps k or v"),
+    ("mc_qk_norm_rope", dict(q_out=0x1000000, q_stride=2560, q_out_stride=2560, v=0x1001400 - 16, v_stride=2560),
+     "overlaps k or v"),
+    ("mc_qk_norm_rope", dict(n_tokens=1, q_out=0x2000000 - 4096 + 16, q_out_stride=1 << 20), "overlaps k or v"),
+    ("mc_qk_norm_rope", dict(q_out=0x4000000, q=0x4001000, q_stride=2040), "overlaps q"),
+    ("mc_qk_norm_rope", dict(q=0x100000), "in the cache"),
+    ("mc_qk_norm_rope", dict(q_out=0x200400), "in the cache"),
+    # a stride whose product with the pages passes 64 bits
+    ("mc_qk_norm_rope", dict(num_blocks=257, block_stride=1 << 62), "2^32"),
+    ("mc_paged_attention", dict(num_blocks=257, block_stride=1 << 62), "2^32"),
+    ("mc_logits_mark", dict(seen=0x202), "misaligned"),
+    ("mc_logits_mark", dict(counts=0x301), "misaligned"),
 ]
 
 
@@ -143,6 +156,10 @@ def test_refusals(lib, name, changed, words):
     ("mc_qk_norm_rope", dict(rot_dim=0, positions=None, turns=None)),
     ("mc_qk_norm_rope", dict(kv_dtype=_lib.DTYPE_E4M3, k_scale=0x600, v_scale=0x700)),
     ("mc_qk_norm_rope", dict(num_blocks=1, block_size=1, block_stride=0)),
+    ("mc_qk_norm_rope", dict(num_blocks=1, block_stride=1 << 62)),           # one page: no distance
+    ("mc_qk_norm_rope", dict(n_kv_heads=4, q_stride=2560, k=0x1001000, k_stride=2560, v=0x1001200, v_stride=2560,
+                             q_out=0x1000000, q_out_stride=2560)),           # in place in a fused row
+    ("mc_qk_norm_rope", dict(q_stride=4608, q_out=0x1001000, q_out_stride=4608)),  # beside q in its rows
     ("mc_paged_attention", dict(row_req=0x500, n_rows=1000)),
     ("mc_paged_attention", dict(n_heads=8)),
     ("mc_logits_process", dict(out=0x1000000)),                              # in place
@@ -214,6 +231,15 @@ def test_python_checks_come_first():
     both = bf(5, 2, 2, 4, 64)
     halves = kv.KvCache(both[:, 0], both[:, 1])
     assert halves._where[2:] == (_lib.DTYPE_BF16, 5, 4, 2 * 2 * 4 * 64)
+    with pytest.raises(ValueError, match="empty"):
+        kv.KvCache(bf(0, 1, 4, 64), bf(0, 1, 4, 64))
+    with pytest.raises(AttributeError):
+        halves.k = bf(5, 2, 4, 64)  # its address is taken
+    with pytest.raises(ValueError, match="rot_dim"):
+        kv.rope_turns(-2)
+    one = torch.zeros(3, 128, dtype=torch.bfloat16).as_strided((1, 2, 64), (101, 64, 1))
+    here = type("Here", (), dict(device=torch.device("cpu"), index=-1))()
+    assert kv._rows(here, one, one.shape, "q") == (one.data_ptr(), 128)  # a single row's stride says nothing
     with pytest.raises(ValueError, match="query heads"):
         kv.paged_attention(ctx, bf(1, 3, 64), halves, i32(1, 5), i32(1), bf(1, 3, 64), i32(4))
     with pytest.raises(ValueError, match="must be on"):
