@@ -31,7 +31,7 @@
 namespace {
 
 constexpr int kMaxThreads = 384;
-constexpr int kBatch = 8;   // most tokens of a CTA
+constexpr int kBatch = 16;   // most tokens of a CTA
 constexpr int kFlight = 4;    // tokens whose loads are in flight together
 constexpr int kResident = 2;  // CTAs an SM holds at once
 
@@ -59,37 +59,69 @@ struct RopeParams {
   uint32_t* status;
 };
 
-__device__ __forceinline__ void unpack4(const uint2& u, float* f) {
-  f[0] = __uint_as_float(u.x << 16);
-  f[1] = __uint_as_float(u.x & 0xffff0000u);
-  f[2] = __uint_as_float(u.y << 16);
-  f[3] = __uint_as_float(u.y & 0xffff0000u);
+// Two floats under one instruction, each rounded as alone.
+struct Two {
+  unsigned long long v;
+};
+__device__ __forceinline__ Two two(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
 }
-
-__device__ __forceinline__ uint2 pack4(const float* f) {
-  uint2 r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r.x) : "f"(f[1]), "f"(f[0]));
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r.y) : "f"(f[3]), "f"(f[2]));
+__device__ __forceinline__ float2 parts(Two a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ Two mul(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
   return r;
 }
 
-__device__ __forceinline__ uint32_t pack4_e4m3(const float* f) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3);
+// 4 elements: the even two and the odd two.
+struct Four {
+  Two even, odd;
+};
+
+__device__ __forceinline__ Four unpack4(const uint2& u) {
+  return {two(__uint_as_float(u.x << 16), __uint_as_float(u.y << 16)),
+          two(__uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y & 0xffff0000u))};
+}
+
+__device__ __forceinline__ uint2 pack4(const Four& f) {
+  const float2 e = parts(f.even), o = parts(f.odd);
+  uint2 r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r.x) : "f"(o.x), "f"(e.x));
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r.y) : "f"(o.y), "f"(e.y));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t pack4_e4m3(const Four& f) {
+  const float2 e = parts(f.even), o = parts(f.odd);
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(e.x, o.x), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(e.y, o.y), __NV_SATFINITE, __NV_E4M3);
   return lo | hi << 16;
 }
 
-__device__ __forceinline__ void rotate(float& a, float& b, float cosine, float sine) {
-  const float p = a;
-  a = __fmaf_rn(p, cosine, -(b * sine));
-  b = __fmaf_rn(b, cosine, p * sine);
+// (a, b) -> (a cos - b sin, b cos + a sin); `minus`: -sin
+__device__ __forceinline__ void rotate(Two& a, Two& b, Two cosine, Two sine, Two minus) {
+  const Two p = a;
+  a = fma2(b, minus, mul(p, cosine));
+  b = fma2(p, sine, mul(b, cosine));
 }
 
 // D: head_dim; F8: e4m3 cache.
 template <int D, bool F8>
 __global__ void __launch_bounds__(kMaxThreads, kResident) qk_norm_rope_kernel(const RopeParams P) {
   constexpr int L = D / 8;  // threads of a row
-  __shared__ __align__(16) float2 cs[kBatch][D / 2];
+  // cosines and sines of a token, those of a thread's 4 pairs together
+  __shared__ __align__(16) float cos_s[kBatch][D / 2], sin_s[kBatch][D / 2];
   __shared__ uint32_t row_s[kBatch];  // the token's row of head 0 in the cache, all ones: none
   const int tid = threadIdx.x, c = tid % L;
   const int half = P.rot / 2, turned = P.rot / 8;  // threads of a row that rotate
@@ -118,23 +150,23 @@ __global__ void __launch_bounds__(kMaxThreads, kResident) qk_norm_rope_kernel(co
   mc_pdl_wait();
 
   uint2 xa[kFlight], xb[kFlight];
-  auto load = [&](int t) {  // tokens t, t + 1, ...
-    const uint16_t* p = src + (size_t)t * stride;
-#pragma unroll
-    for (int i = 0; i < kFlight; ++i) {
-      if (in && t + i < t_end) {
-        // plain loads: q_out may be q
-        xa[i] = *reinterpret_cast<const uint2*>(p + 4 * a);
-        xb[i] = *reinterpret_cast<const uint2*>(p + 4 * b);
-      }
-      p += stride;
+  int coming = in ? t_end - t0 : 0;  // tokens that are still to be asked for, the next at src
+  src += (size_t)t0 * stride;
+  auto load = [&](int i) {
+    if (coming > 0) {
+      // plain loads: q_out may be q
+      xa[i] = *reinterpret_cast<const uint2*>(src + 4 * a);
+      xb[i] = *reinterpret_cast<const uint2*>(src + 4 * b);
     }
+    --coming;
+    src += stride;
   };
-  load(t0);
-  float ga[4], gb[4];
+#pragma unroll
+  for (int i = 0; i < kFlight; ++i) load(i);
+  Four ga, gb;
   if (in && w) {
-    unpack4(__ldg(reinterpret_cast<const uint2*>(w) + a), ga);
-    unpack4(__ldg(reinterpret_cast<const uint2*>(w) + b), gb);
+    ga = unpack4(__ldg(reinterpret_cast<const uint2*>(w) + a));
+    gb = unpack4(__ldg(reinterpret_cast<const uint2*>(w) + b));
   }
   float scale = 1.0f;
   if (F8 && in && !is_q) {
@@ -152,7 +184,11 @@ __global__ void __launch_bounds__(kMaxThreads, kResident) qk_norm_rope_kernel(co
       const float x = __ll2float_rn((long long)turn) * 1.0842021724855044e-19f;  // 2^-63
       float s, co;
       sincospif(x, &s, &co);
-      cs[t][f] = make_float2(co, s);
+      // a thread's pairs 0 1 2 3 stand as two words of two that rotate under one instruction:
+      // 0 2 and 1 3, interleaved 0 1 and 2 3
+      const int at = P.interleaved || f % 4 == 0 || f % 4 == 3 ? f : f ^ 3;
+      cos_s[t][at] = co;
+      sin_s[t][at] = s;
     }
     if (tid < n) {
       const unsigned long long slot = P.slots ? P.slots[t0 + tid] : (unsigned long long)(t0 + tid);
@@ -171,38 +207,34 @@ __global__ void __launch_bounds__(kMaxThreads, kResident) qk_norm_rope_kernel(co
 #pragma unroll
       for (int i = 0; i < kFlight; ++i) {
         if (t + i >= n) break;  // the same for the whole CTA
-        float x[4], y[4];
-        unpack4(xa[i], x);
-        unpack4(xb[i], y);
+        Four x = unpack4(xa[i]), y = unpack4(xb[i]);
+        load(i);
         if (P.qw || P.kw) {
-          float ss = 0.0f;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) ss = __fmaf_rn(x[j], x[j], __fmaf_rn(y[j], y[j], ss));
+          const float2 sum = parts(fma2(
+              x.even, x.even,
+              fma2(x.odd, x.odd, fma2(y.even, y.even, mul(y.odd, y.odd)))));
+          float ss = sum.x + sum.y;
 #pragma unroll
           for (int m = 1; m < L; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
           if (w) {
-            const float inv = rsqrtf(__fmaf_rn(ss, 1.0f / D, P.eps));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              x[j] = x[j] * inv * ga[j];
-              y[j] = y[j] * inv * gb[j];
-            }
+            const float one = rsqrtf(__fmaf_rn(ss, 1.0f / D, P.eps));
+            const Two inv = two(one, one);
+            x = {mul(mul(x.even, inv), ga.even), mul(mul(x.odd, inv), ga.odd)};
+            y = {mul(mul(y.even, inv), gb.even), mul(mul(y.odd, inv), gb.odd)};
           }
         }
         if (turns_here) {
           // this thread's four frequencies: 4 c .. 4 c + 3
-          const float4 e = *reinterpret_cast<const float4*>(&cs[t + i][4 * c]);
-          const float4 f = *reinterpret_cast<const float4*>(&cs[t + i][4 * c + 2]);
+          const float4 e = *reinterpret_cast<const float4*>(&cos_s[t + i][4 * c]);
+          const float4 f = *reinterpret_cast<const float4*>(&sin_s[t + i][4 * c]);
+          const Two c0 = two(e.x, e.y), c1 = two(e.z, e.w), s0 = two(f.x, f.y), s1 = two(f.z, f.w);
+          const Two m0 = two(-f.x, -f.y), m1 = two(-f.z, -f.w);
           if (P.interleaved) {
-            rotate(x[0], x[1], e.x, e.y);
-            rotate(x[2], x[3], e.z, e.w);
-            rotate(y[0], y[1], f.x, f.y);
-            rotate(y[2], y[3], f.z, f.w);
+            rotate(x.even, x.odd, c0, s0, m0);
+            rotate(y.even, y.odd, c1, s1, m1);
           } else {
-            rotate(x[0], y[0], e.x, e.y);
-            rotate(x[1], y[1], e.z, e.w);
-            rotate(x[2], y[2], f.x, f.y);
-            rotate(x[3], y[3], f.z, f.w);
+            rotate(x.even, y.even, c0, s0, m0);
+            rotate(x.odd, y.odd, c1, s1, m1);
           }
         }
         if (!in) continue;
@@ -213,11 +245,9 @@ __global__ void __launch_bounds__(kMaxThreads, kResident) qk_norm_rope_kernel(co
         } else if (row_s[t + i] != 0xffffffffu) {
           const size_t at = (size_t)(row_s[t + i] + head_row) * D;
           if (F8) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              x[j] *= scale;
-              y[j] *= scale;
-            }
+            const Two by = two(scale, scale);
+            x = {mul(x.even, by), mul(x.odd, by)};
+            y = {mul(y.even, by), mul(y.odd, by)};
             uint8_t* to = static_cast<uint8_t*>(cache) + at;
             *reinterpret_cast<uint32_t*>(to + 4 * a) = pack4_e4m3(x);
             *reinterpret_cast<uint32_t*>(to + 4 * b) = pack4_e4m3(y);
@@ -228,7 +258,6 @@ __global__ void __launch_bounds__(kMaxThreads, kResident) qk_norm_rope_kernel(co
           }
         }
       }
-      load(t0 + min(t + kFlight, n));
     }
   }
 }
@@ -244,7 +273,8 @@ int launch_rope(mc_ctx* ctx, RopeParams& P) {
   const int wave = kResident * ctx->num_sms, slots = wave > parts ? wave / parts : 1;
   P.share = (P.tokens + slots - 1) / slots;
   const int batches = (P.share + kBatch - 1) / kBatch;
-  P.batch = (P.share + batches - 1) / batches;
+  // whole rounds of the tokens in flight, so that a token keeps its place among them
+  P.batch = ((P.share + batches - 1) / batches + kFlight - 1) / kFlight * kFlight;
   const dim3 grid((unsigned)((P.tokens + P.share - 1) / P.share), (unsigned)parts);
   MC_CUDA(mc_launch_pdl(qk_norm_rope_kernel<D, F8>, grid, dim3(threads), 0, ctx->stream, P));
   return mc_after_launch("qk_norm_rope_kernel");
