@@ -20,9 +20,11 @@
 // the CTA's batch: its gains, addresses and role stay in registers. A batch's
 // cosines, sines and cache rows are computed once into shared memory by all
 // threads together. One wave of CTAs shares the tokens evenly, in batches of
-// up to 8, with the loads of the next 4 in flight (4096 tokens of 32 + 2 x 8
-// heads of 64, 50 MB, mostly in L2: 15 us; 3 CTAs an SM with fewer loads each
-// 15.5 us; a CTA a token, rotation partners by shuffle, 25.6 us).
+// up to 16, with 4 tokens' loads in flight, each asked for as soon as the one
+// in its place is unpacked (4096 tokens of 32 + 2 x 8 heads of 64, 50 MB from
+// HBM: 12.7 us; 4 loaded together after 4 are done, in batches of 8, 14.6; 3
+// CTAs an SM with 2 in flight each 13.0; a CTA a token, rotation partners by
+// shuffle, 25.6).
 #include <cuda_fp8.h>
 #include <math.h>
 
