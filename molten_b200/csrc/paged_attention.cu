@@ -269,6 +269,10 @@ paged_attention_kernel(const PaParams P) {
       if (P.row_req && (P.row_req[r] < -1 || P.row_req[r] >= P.n_req))
         atomicOr(P.status, MC_KV_BAD_ROW);
     }
+  const int cost = ps_cost(U, factor, gridDim.x);
+  mine += cost * P.items * (r_hi - r_lo);
+  incl += cost * P.items * r_hi;
+  U += cost * P.items * P.rows;
   const int G = min((int)gridDim.x, U);
   if (cta >= G) return;
   const int u0 = ps_begin(U, cta, G), u_end = ps_begin(U, cta + 1, G);
@@ -277,7 +281,7 @@ paged_attention_kernel(const PaParams P) {
   const bool here = u0 >= row_at && u0 < incl;
   if (here) {
     for (; row0 < r_hi - 1; ++row0) {
-      const int n = units_of(row0) * P.items;
+      const int n = (units_of(row0) + cost) * P.items;
       if (u0 < row_at + n) break;
       row_at += n;
     }
@@ -288,7 +292,8 @@ paged_attention_kernel(const PaParams P) {
 
   // ---- filling the ring: the step at fill_base of the piece `fill`
   uint8_t* ring = ring_s + (size_t)warp * S::kStages * S::kStage;
-  PsCursor fill = ps_first(row0, u0 - row_at, units_of(row0), P.items, u_end - u0);
+  PsCursor fill = ps_first(row0, u0 - row_at, units_of(row0), P.items, u_end - u0, cost);
+  if (fill.units <= 0) return;  // no more than an item's start
   PsCursor piece = fill;
   int fill_base = 0, fill_hi = 0, fill_stage = 0, page = -1;
   uint32_t in_page = 0, head_row = 0;

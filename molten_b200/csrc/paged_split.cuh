@@ -9,9 +9,10 @@
 // is a run of pieces, one for each item it touches; an item whole inside one
 // CTA is written at once, one that spans several CTAs is joined from their
 // partial results. Where the items are alike enough, the unit is made so long
-// that every CTA has one piece (ps_factor). The host chooses the smallest unit
-// so that there are fewer than 2^31 (ps_small_unit): the arithmetic is in 32
-// bits.
+// that every CTA has one piece (ps_factor). Elsewhere the start of an item
+// counts as units of its own that hold no keys (ps_cost), so that a CTA with
+// many short pieces gets fewer keys. The host chooses the smallest unit so that
+// there are fewer than 2^31 (ps_small_unit): the arithmetic is in 32 bits.
 #pragma once
 #include <stdint.h>
 
@@ -65,12 +66,19 @@ PS_HD int ps_units(PsRow r, int unit) {
   return n <= (uint32_t)unit ? 1 : (int)((n + (uint32_t)unit - 1) / (uint32_t)unit);
 }
 
+// What the start of an item counts as, in units: a CTA with one piece was done
+// with its keys 2.6 us before one with two, 16 to 32 KB of keys take 1.1 to 1.5
+// (ps_cost). 32 rows of 17 to 6000 keys of 64: 42.7 us with 0, 41.1, 40.9, 41.1
+// with 1, 2, 3; 60 rows up to 1500: 29.7, 27.0, 27.4, 28.1; 64 e4m3 rows of 17 to
+// 8200 keys of 128: 117.1, 109.0, 107.8, 108.5.
+constexpr int kPsCost = 2;
+
 // The smallest unit, `unit` times a power of two, with which `items` items of
-// up to `capacity` keys have fewer than 2^31 units; 0: none.
+// up to `capacity` keys have fewer than 2^31 units with their starts; 0: none.
 inline int ps_small_unit(int unit, long long items, int capacity) {
   for (long long u = unit; u < 0x40000000; u *= 2) {
     const long long n = ((long long)capacity + u - 1) / u;
-    if (items <= 0x7fffffffll / (n < 1 ? 1 : n)) return (int)u;
+    if (items <= 0x7fffffffll / ((n < 1 ? 1 : n) + kPsCost)) return (int)u;
   }
   return 0;
 }
@@ -92,6 +100,12 @@ PS_HD int ps_factor(int U, int n_max, int items, int slots) {
   return (f - 2) * slots <= U ? f : 1;  // (f - 2) slots < 2 n_max items + slots
 }
 
+// Units that the start of an item counts as: none where CTAs have a unit or
+// two, or one piece each (`factor` above 1).
+PS_HD int ps_cost(int U, int factor, int slots) {
+  return factor == 1 && U / 2 >= slots ? kPsCost : 0;
+}
+
 // floor(U c / G), G <= 1024, 0 <= c <= G.
 PS_HD int ps_begin(int U, int c, int G) {
   const uint32_t q = (uint32_t)U / (uint32_t)G, r = (uint32_t)U - q * (uint32_t)G;  // r c <= 2^20
@@ -105,25 +119,31 @@ PS_HD int ps_owner(int u, int U, int G) {
 }
 
 // Walks the pieces of one CTA: the item, its units in this CTA, and how many
-// units of the range are left from the piece's first one on.
+// units of the range are left from the piece's first one on. Counted with the
+// items' starts, the first unit of the piece's item is unit (end of the range)
+// - left - unit.
 struct PsCursor {
   int row, item;    // query row, item within the row
   int n;            // units of each of the row's items
   int unit, units;  // first unit of the piece within the item, unit count
   int left;
+  int cost;         // units of an item's start
 };
 
 // The piece that starts `in_row` units after the start of row `row` (n units
-// an item), with `left` units of the range to go.
-PS_HD PsCursor ps_first(int row, int in_row, int n, int items, int left) {
+// an item and `cost` for its start), with `left` units of the range to go. Not
+// above 0 units: the range holds no more than (a part of) a start.
+PS_HD PsCursor ps_first(int row, int in_row, int n, int items, int left, int cost = 0) {
   PsCursor c;
   c.row = row;
   c.n = n;
-  const int item = (int)((uint32_t)in_row / (uint32_t)n);
+  c.cost = cost;
+  const int each = n + cost, item = (int)((uint32_t)in_row / (uint32_t)each);
   c.item = item < items ? item : items - 1;
-  c.unit = item < items ? in_row - item * n : n - 1;
-  c.left = left;
-  c.units = left < n - c.unit ? left : n - c.unit;
+  const int in_item = (item < items ? in_row - item * each : each - 1) - cost;
+  c.unit = in_item < 0 ? 0 : in_item;
+  c.left = in_item < 0 ? left + in_item : left;
+  c.units = c.left < n - c.unit ? c.left : n - c.unit;
   return c;
 }
 
@@ -133,7 +153,7 @@ PS_HD PsCursor ps_first(int row, int in_row, int n, int items, int left) {
 // after `items` items; units_of(row) gives the next row's n.
 template <typename F>
 PS_HD bool ps_next(PsCursor& c, int items, int rows, F&& units_of) {
-  c.left -= c.units;
+  c.left -= c.units + c.cost;
   if (c.left <= 0) return false;
   c.unit = 0;
   if (++c.item == items) {
