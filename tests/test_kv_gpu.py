@@ -366,6 +366,26 @@ def test_attention(cuda_ctx, lens, H, K, D, bs, fp8, window):
     assert not ws[:2048].any(), "the joining counters are zero again"
 
 
+@pytest.mark.parametrize("lens,H,K,D,bs,fp8,window", [
+    ([20000] + 200 * [0], 8, 2, 64, 16, False, 0),            # one long row among empty ones
+    (90 * [1, 130, 0, 700], 4, 2, 64, 16, True, 0),           # many short pieces in a CTA
+    ([3000, 17, 2500, 1, 900, 6000, 0, 40] * 6, 8, 4, 128, 24, False, 0),
+    ([3000, 17, 2500, 1, 900, 6000, 0, 40] * 9, 16, 8, 64, 16, True, 1000),
+    ([129 * i % 5000 for i in range(40)], 32, 2, 64, 32, False, 0),  # 16 heads a tile
+])
+def test_attention_pieces_of_unlike_rows(cuda_ctx, lens, H, K, D, bs, fp8, window):
+    """Batches whose split counts the starts of the pieces."""
+    q, c, table, keys = attention_case(len(lens) + D, lens, H, K, D, bs, fp8)
+    out = torch.full_like(q, NAN)
+    lse = torch.full((len(lens), H), NAN, device="cuda")
+    st = torch.zeros(1, dtype=I32, device="cuda")
+    ws = kv.paged_attention_workspace(D)
+    for _ in range(2):  # the second finds the counters as the first left them
+        kv.paged_attention(cuda_ctx, q, c, table, i32(lens), out, ws, window=window, lse=lse, status=st)
+    assert st.item() == 0
+    check_attention(out, lse, q, keys, lens, window=window)
+
+
 def test_attention_strided_rows_and_halves(cuda_ctx):
     lens, H, K, D, bs = [100, 3, 777, 0], 8, 2, 64, 16
     q, cache, table, keys = attention_case(1, lens, H, K, D, bs, halves=True)
