@@ -869,12 +869,12 @@ extern "C" int mc_paged_attention(mc_ctx* ctx, const uint16_t* q, size_t q_strid
   MC_CUDA(dev.error());
   const long long capacity = (long long)table_width * block_size;
   PaParams P{q, q_stride, n_rows, n_heads, n_kv_heads, n_heads / n_kv_heads, 0, 0,
-                   k_cache, v_cache, num_blocks, block_size, (uint32_t)(block_stride / head_dim),
-                   ps_div_of(block_size), k_scale, v_scale, block_table, n_req, table_width,
-             (int)(capacity < 0x7fff0000ll ? capacity : 0x7fff0000ll), 0, kv_lens, row_req, window, scale * kLog2e,
-                   out, out_stride, lse, static_cast<uint32_t*>(workspace),
-                   reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes), status,
-                   mc_wait_limit(ctx, 1000000000ull),
+             k_cache, v_cache, num_blocks, block_size, (uint32_t)(block_stride / head_dim),
+             ps_div_of(block_size), k_scale, v_scale, block_table, n_req, table_width,
+             (int)(capacity < 0x7fff0000ll ? capacity : 0x7fff0000ll), 0, kv_lens, row_req, window,
+             scale * kLog2e, out, out_stride, lse, static_cast<uint32_t*>(workspace),
+             reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes), status,
+             mc_wait_limit(ctx, 1000000000ull),
              (ctx->test_flags & MC_TEST_SKIP_KV_ARRIVE) ? 1 : 0};
   const bool f8 = kv_dtype == MC_DTYPE_E4M3;
   if (head_dim == 64)
