@@ -36,6 +36,7 @@ pub const MC_KV_WAIT: c_int = 256;
 pub const MC_TEST_SKIP_LOGIT_PUBLISH: c_int = 1;
 pub const MC_TEST_SKIP_BARRIER_ARRIVE: c_int = 2;
 pub const MC_TEST_SKIP_KV_ARRIVE: c_int = 4;
+pub const MC_TEST_LATE_KV_ARRIVE: c_int = 8;
 
 /// mc_ctx: opaque (one device and stream; expert-parallel state).
 #[repr(C)]

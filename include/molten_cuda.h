@@ -675,6 +675,9 @@ int mc_set_wait_limit(mc_ctx* ctx, unsigned long long ns);
 /* MC_TEST_SKIP_KV_ARRIVE: one warp of mc_paged_attention waits for copies that
  * it does not report as arrived, so its wait runs out and sets MC_KV_WAIT. */
 #define MC_TEST_SKIP_KV_ARRIVE 4
+/* MC_TEST_LATE_KV_ARRIVE: one lane of that warp gives up at once, and what the
+ * others wait for is reported after it has. */
+#define MC_TEST_LATE_KV_ARRIVE 8
 int mc_set_test_flags(mc_ctx* ctx, int flags);
 
 /* Evaluates the library's device math on x[n] into y[n]: op 0 = mc_exp,

@@ -21,6 +21,7 @@ MC_ETIMEOUT = -5
 TEST_SKIP_LOGIT_PUBLISH = 1
 TEST_SKIP_BARRIER_ARRIVE = 2
 TEST_SKIP_KV_ARRIVE = 4
+TEST_LATE_KV_ARRIVE = 8
 
 ROUTE_SOFTMAX_RENORM = 0
 ROUTE_SIGMOID_BIAS = 1

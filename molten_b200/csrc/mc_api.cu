@@ -118,7 +118,8 @@ extern "C" int mc_set_wait_limit(mc_ctx* ctx, unsigned long long ns) {
 
 extern "C" int mc_set_test_flags(mc_ctx* ctx, int flags) {
   if (!ctx) return mc_fail(MC_EINVAL, "mc_set_test_flags: null context");
-  if (flags & ~(MC_TEST_SKIP_LOGIT_PUBLISH | MC_TEST_SKIP_BARRIER_ARRIVE | MC_TEST_SKIP_KV_ARRIVE))
+  if (flags & ~(MC_TEST_SKIP_LOGIT_PUBLISH | MC_TEST_SKIP_BARRIER_ARRIVE | MC_TEST_SKIP_KV_ARRIVE |
+                MC_TEST_LATE_KV_ARRIVE))
     return mc_fail(MC_EINVAL, "mc_set_test_flags: unknown flags 0x%x", flags);
   ctx->test_flags = flags;
   return MC_OK;

@@ -89,7 +89,8 @@ struct PaParams {
   float* parts;
   uint32_t* status;
   unsigned long long wait_ns;
-  int skip_arrive;  // test aid (mc_set_test_flags): a warp's copies are never reported as arrived
+  int skip_arrive;  // test aids (mc_set_test_flags): a warp's copies are never reported as arrived
+                    // (1), or by a lane that has given up on them (2)
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -131,15 +132,25 @@ __device__ __forceinline__ float2 unpack2(uint32_t u) {
   return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
 
-// Waits (every lane polls) for a stage's bytes; false after `limit_ns`.
-__device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity,
-                                          unsigned long long limit_ns) {
-  if (mc_mbar_test(bar, parity)) return true;
-  const unsigned long long t0 = mc_globaltimer();
-  do {
-    if (mc_mbar_test_sleep(bar, parity, limit_ns < 1000 ? (uint32_t)limit_ns : 1000)) return true;
-  } while (mc_globaltimer() - t0 < limit_ns);
-  return false;
+// Waits (every lane polls) for a stage's bytes. False, for the whole warp alike, if any lane's wait
+// ran past `limit_ns`: what follows takes all lanes together. A lane with `late` (a test's) gives up
+// at once and reports then what the other lanes wait for.
+__device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity, unsigned long long limit_ns,
+                                          bool late) {
+  bool ok = mc_mbar_test(bar, parity);
+  if (!ok) {
+    const unsigned long long t0 = mc_globaltimer();
+    const unsigned long long limit = late ? 0 : limit_ns;
+    for (;;) {
+      ok = mc_mbar_test_sleep(bar, parity, limit < 1000 ? (uint32_t)limit : 1000);
+      if (ok) break;
+      if (mc_globaltimer() - t0 >= limit) {
+        if (late) mc_mbar_arrive(bar);
+        break;
+      }
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
 }
 
 // Four e4m3 bytes -> two f16 pairs (exact).
@@ -213,7 +224,8 @@ paged_attention_kernel(const PaParams P) {
   __shared__ float m_s[S::kWarps][kHeads], l_s[S::kWarps][kHeads];
   __shared__ uint32_t last_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // a warp's own barriers, an arrival a lane (33 never come: a test's wait that runs out)
+  // a warp's own barriers, an arrival a lane (of 33 the last never comes, or late: a test's wait
+  // that runs out)
   if (lane < S::kStages)
     mc_mbar_init(&full_s[warp][lane], P.skip_arrive && blockIdx.x == 0 && warp == 0 ? 33 : 32);
   mc_fence_barrier_init();
@@ -472,7 +484,8 @@ paged_attention_kernel(const PaParams P) {
     float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // sums of P, a product with a column of ones
 
     for (int base = lo + warp * S::kStep; base < hi; base += S::kUnit) {
-      if (!wait_full(&full_s[warp][stage], phase, gave_up ? 0 : P.wait_ns)) {
+      if (!wait_full(&full_s[warp][stage], phase, gave_up ? 0 : P.wait_ns,
+                     P.skip_arrive == 2 && !gave_up && cta == 0 && tid == 5)) {
         gave_up = true;  // nothing more is issued: the stage's barrier may still be open
         more = false;
         if (lane == 0 && P.status) atomicOr(P.status, MC_KV_WAIT);
@@ -875,7 +888,9 @@ extern "C" int mc_paged_attention(mc_ctx* ctx, const uint16_t* q, size_t q_strid
              scale * kLog2e, out, out_stride, lse, static_cast<uint32_t*>(workspace),
              reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes), status,
              mc_wait_limit(ctx, 1000000000ull),
-             (ctx->test_flags & MC_TEST_SKIP_KV_ARRIVE) ? 1 : 0};
+             ctx->test_flags & MC_TEST_SKIP_KV_ARRIVE   ? 1
+             : ctx->test_flags & MC_TEST_LATE_KV_ARRIVE ? 2
+                                                        : 0};
   const bool f8 = kv_dtype == MC_DTYPE_E4M3;
   if (head_dim == 64)
     return f8 ? launch_attention<64, true>(ctx, P) : launch_attention<64, false>(ctx, P);
