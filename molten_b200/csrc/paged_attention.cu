@@ -138,6 +138,7 @@ __device__ __forceinline__ float2 unpack2(uint32_t u) {
 __device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity, unsigned long long limit_ns,
                                           bool late) {
   bool ok = mc_mbar_test(bar, parity);
+  if (__all_sync(0xffffffffu, ok)) return true;
   if (!ok) {
     const unsigned long long t0 = mc_globaltimer();
     const unsigned long long limit = late ? 0 : limit_ns;
