@@ -29,7 +29,13 @@
 //
 // Rounding of P. P is split into high and low parts (bf16 + bf16, or f16 + f16
 // for an e4m3 cache), so it enters the product with 16 bits or more and the
-// output's own rounding is the only one that counts. Eight heads fill rows 0-7
+// output's own rounding is the only one that counts. f16's last step is 2^-24:
+// for an e4m3 cache the running maximum is taken 15 powers of two lower, so
+// that the largest weight is 2^15, and weights have 16 bits down to 2^-24 of
+// the largest one of the warp's keys, fewer below, and none below 2^-40 (with
+// a largest weight of 1 a key of weight 2^-25 counted nothing, and one that
+// outweighs a long flat tail but has V near zero left a result that was off by
+// its own size). Eight heads fill rows 0-7
 // of the 16-row tile, and the low parts ride in rows 8-15 at no cost; where
 // more than 8 heads share a KV head a tile takes 16 and the low parts cost
 // products of their own (16 heads a KV head, 64 rows of 4000 to 8200 keys of
@@ -58,6 +64,8 @@ namespace {
 constexpr int kMaxCtas = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+// The weights of an e4m3 cache's keys are 2^kUp times exp(s - max s), the most that f16 holds.
+constexpr float kUp = 15.0f, kDown = 0x1p-15f;
 
 // A piece's partial result in the workspace: o[heads][D], m[heads], l[heads] (8 or 16 heads).
 constexpr size_t part_floats(int D, int heads) { return (size_t)heads * D + 2 * heads; }
@@ -384,7 +392,12 @@ paged_attention_kernel(const PaParams P) {
                    (kHalfChunk ? 16 * ((hr >> 1) ^ (2 * c)) + 8 * (hr & 1) : 16 * (hr ^ (2 * c)));
   const int v_flip = (v_at ^ 64) - v_at;
   // Four elements of an item's result (quad `at`: head 4 at / D of the item) from their sums.
-  auto finish = [&](int row, int head0, float vscale, int at, float mx, float sum, const float4& v) {
+  auto finish = [&](int row, int head0, float vscale, int at, float mx, float sum, float4 v) {
+    if (F8) {
+      mx += kUp;
+      sum *= kDown;
+      v = make_float4(v.x * kDown, v.y * kDown, v.z * kDown, v.w * kDown);
+    }
     const int head = head0 + 4 * at / D, d = 4 * at % D;
     const float by = sum == 0.0f ? 0.0f : __fdiv_rn(vscale, sum);  // NaN of a zero sum: 0
     uint2 r;
@@ -548,7 +561,8 @@ paged_attention_kernel(const PaParams P) {
           top = fmaxf(top, fmaxf(fmaxf(t[u][z][0], t[u][z][1]), fmaxf(t[u][z][2], t[u][z][3])));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        m_new[u] = fmaxf(m[u], top * qk[u]);
+        // e4m3: see kUp; both roundings go up, so that no weight passes 2^kUp
+        m_new[u] = fmaxf(m[u], F8 ? __fadd_ru(__fmul_ru(top, qk[u]), -kUp) : top * qk[u]);
         m_use[u] = m_new[u] == -INFINITY ? 0.0f : m_new[u];
         grown |= m_new[u] != m[u];
       }
