@@ -73,6 +73,7 @@ extern "C" {
     pub fn mc_create(device: c_int, stream: *mut c_void, out: *mut *mut McCtx) -> c_int;
     pub fn mc_destroy(ctx: *mut McCtx) -> c_int;
     pub fn mc_set_stream(ctx: *mut McCtx, stream: *mut c_void) -> c_int;
+    pub fn mc_stream_slot(ctx: *const McCtx) -> *const *mut c_void;
     pub fn mc_sync(ctx: *mut McCtx) -> c_int;
     pub fn mc_last_error() -> *const c_char;
     pub fn mc_version() -> *const c_char;

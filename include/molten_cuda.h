@@ -85,6 +85,10 @@ int mc_create(int device, void* stream, mc_ctx** out);
 int mc_destroy(mc_ctx* ctx);
 /* Switches the stream later calls enqueue on (NULL = the default stream). */
 int mc_set_stream(mc_ctx* ctx, void* stream);
+/* Where the context holds its stream, for a host that looks before each call
+ * whether it has to switch (read only, until mc_destroy; NULL of a NULL
+ * context). */
+void* const* mc_stream_slot(const mc_ctx* ctx);
 /* ComputePass::commit_wait (metal.rs:383-399): waits for all enqueued work
  * and reports any asynchronous CUDA error. */
 int mc_sync(mc_ctx* ctx);

@@ -82,6 +82,7 @@ SIGNATURES: dict[str, tuple] = {
     "mc_create": (I, [I, P, C.POINTER(P)]),
     "mc_destroy": (I, [P]),
     "mc_set_stream": (I, [P, P]),
+    "mc_stream_slot": (P, [P]),
     "mc_sync": (I, [P]),
     "mc_last_error": (C.c_char_p, []),
     "mc_version": (C.c_char_p, []),

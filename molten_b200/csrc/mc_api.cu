@@ -102,6 +102,10 @@ extern "C" int mc_set_stream(mc_ctx* ctx, void* stream) {
   return MC_OK;
 }
 
+extern "C" void* const* mc_stream_slot(const mc_ctx* ctx) {
+  return ctx ? reinterpret_cast<void* const*>(&ctx->stream) : nullptr;
+}
+
 extern "C" int mc_set_trace(mc_ctx* ctx, unsigned long long* buf, int n) {
   if (!ctx) return mc_fail(MC_EINVAL, "mc_set_trace: null context");
   if (buf && n < 0) return mc_fail(MC_EINVAL, "mc_set_trace: n %d", n);

@@ -72,18 +72,20 @@ class Context:
         self._fixed_stream = stream
         h = _lib.C.c_void_p()
         s = (stream or torch.cuda.current_stream(dev)).cuda_stream
+        self._fixed = None if stream is None else s
         _lib.check(_lib.lib().mc_create(dev.index or 0, s, _lib.C.byref(h)))
         self.h = h
-        self._stream = s  # the library's context has this one
+        # the word in which the library's context holds its stream: read before each call, since
+        # mc_set_stream may also be called by others (half a microsecond less than calling it)
+        self._slot = _lib.C.c_void_p.from_address(_lib.lib().mc_stream_slot(h))
 
     @property
     def handle(self):
-        if self._fixed_stream is not None:
-            return self.h
-        s = _raw_stream(self.index)
-        if s != self._stream:
+        s = self._fixed
+        if s is None:
+            s = _raw_stream(self.index)
+        if (self._slot.value or 0) != s or not self.h:
             _lib.check(_lib.lib().mc_set_stream(self.h, s))
-            self._stream = s
         return self.h
 
     @property
@@ -116,6 +118,7 @@ class Context:
 
     def close(self) -> None:
         if self.h:
+            self._slot = _lib.C.c_void_p()  # the library's goes with the context
             _lib.lib().mc_destroy(self.h)
             self.h = None
 
