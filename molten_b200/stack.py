@@ -75,6 +75,13 @@ class DecodeStack:
         lfm.ensure(self.path in ("fused", "grouped", "gemv"), f"moe_path {self.path!r}")
         lfm.ensure(self.path != "fused" or batch == 1, "the fused layer is batch 1")
         self.fuse_proj = fuse_proj and self.path == "fused"
+        # the buffers are zeroed on the stream that the steps run on
+        with torch.cuda.stream(ctx.stream):
+            self._allocate(kv, rules, rope_theta)
+
+    def _allocate(self, kv: paged.PagedBatch | None, rules, rope_theta: float) -> None:
+        ctx, layers, head, embed, batch, n_experts, sampling = (
+            self.ctx, self.layers, self.head, self.embed, self.B, self.E, self.sampling)
         H = embed.shape[1]
         I = layers[0]["gate"].out_features // n_experts
         dev = embed.device
@@ -134,11 +141,18 @@ class DecodeStack:
     def start(self, tokens: torch.Tensor, pos: int = 0, seen=()) -> None:
         """Loads the embedding rows of the first tokens (int32 [B]); with
         sampling, ``pos`` is the absolute position of the token the next step
-        draws and ``seen`` the sequence's token ids so far."""
-        self.x.copy_(self.embed[tokens.long()])
-        if self.sample is not None:
-            self.pos.fill_(pos)
-            self.sample.upload_seen(list(seen) + [int(t) for t in tokens.cpu()])
+        draws and ``seen`` the sequence's token ids so far. A context with a
+        stream of its own waits for the current one, where ``tokens`` were made."""
+        stream, current = self.ctx.stream, torch.cuda.current_stream(self.ctx.device)
+        if stream != current:
+            stream.wait_stream(current)
+            if tokens.is_cuda:
+                tokens.record_stream(stream)
+        with torch.cuda.stream(stream):
+            self.x.copy_(self.embed[tokens.long()])
+            if self.sample is not None:
+                self.pos.fill_(pos)
+                self.sample.upload_seen(list(seen) + [int(t) for t in tokens.cpu()])
 
     def _attend(self, A: dict, cur: torch.Tensor) -> torch.Tensor:
         """The attention of one layer on the rows ``cur``: [B, 2048]."""
@@ -222,15 +236,17 @@ class DecodeStack:
     def check(self) -> None:
         """Waits for the stream and raises McError if any kernel of the steps
         run so far reported a wait that ran out (the tokens are then invalid)."""
-        for w in self.status_words():
-            lfm.raise_on_status(w, f"decode stack ({self.path})")
+        with torch.cuda.stream(self.ctx.stream):
+            for w in self.status_words():
+                lfm.raise_on_status(w, f"decode stack ({self.path})")
         if self.attn is not None:
             self.kv.check()
 
     def read_tokens(self) -> torch.Tensor:
         """The last step's tokens on the host, after check()."""
         self.check()
-        return self.tokens.cpu()
+        with torch.cuda.stream(self.ctx.stream):
+            return self.tokens.cpu()
 
     def launches_per_step(self) -> int:
         per_layer = {"fused": 1 if self.fuse_proj else 2, "gemv": 4,
