@@ -122,6 +122,8 @@ class DecodeStack:
                 lfm.ensure(A["cache"].head_dim == D and A["cache"].n_kv_heads == K and
                            A["qkv"].out_features == (heads + 2 * K) * D and heads * D == H and
                            A["cache"].block_size == kv.block_size, "attention layer shapes")
+                lfm.ensure(A["cache"].k.shape[0] >= kv.free_list.numel(),
+                           "an attention layer's cache has fewer pages than the PagedBatch")
             rows = bf(batch, (heads + 2 * K) * D)
             part = lambda a, n: rows[:, a * D:(a + n) * D].view(batch, n, D)  # noqa: E731
             self.attn = dict(normed=bf(batch, H), rows=rows, q=part(0, heads), k=part(heads, K),

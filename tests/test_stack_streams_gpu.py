@@ -53,3 +53,17 @@ def test_a_stack_on_a_stream_of_its_own(cuda_ctx, B, path, with_rules, sampled):
     finally:
         torch.cuda.synchronize()
         ctx.close()
+
+
+def test_a_cache_with_fewer_pages_than_the_batch_is_refused(cuda_ctx):
+    """Any one of the layers; a cache with more pages is fine."""
+    layers, head, embed = make_layers(420, 2, (0, 1), 5, torch.bfloat16)
+    build = lambda pages: DecodeStack(cuda_ctx, layers, head, embed, 1, n_experts=E,  # noqa: E731
+                                      kv=kv.PagedBatch(cuda_ctx, 1, pages, BS, 5))
+    with pytest.raises(ValueError, match="fewer pages"):
+        build(6)
+    build(5)
+    layers[1]["attn"]["cache"] = kv.KvCache.empty(4, 8, BS)
+    with pytest.raises(ValueError, match="fewer pages"):
+        build(5)
+    build(4)
