@@ -93,6 +93,11 @@ class Context:
         """The stream the context enqueues on: its own, or else the current one."""
         return self._fixed_stream or torch.cuda.current_stream(self.device)
 
+    def same_stream(self, other: "Context") -> bool:
+        """The two enqueue on one stream of one device at any time: both on the
+        current one, or both on the same stream of their own."""
+        return self.index == other.index and self._fixed == other._fixed
+
     def commit_wait(self) -> None:
         _lib.check(_lib.lib().mc_sync(self.h))
 

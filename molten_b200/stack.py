@@ -115,6 +115,7 @@ class DecodeStack:
         if with_attn:
             lfm.ensure(kv.lens.numel() == batch and kv.slots.numel() == batch,
                        "the PagedBatch has one token row for each row of the batch")
+            lfm.ensure(kv.ctx.same_stream(ctx), "the PagedBatch's context enqueues on another stream")
             c = with_attn[0]["cache"]
             D, K = c.head_dim, c.n_kv_heads
             heads = with_attn[0]["qkv"].out_features // D - 2 * K

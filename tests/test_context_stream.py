@@ -74,6 +74,14 @@ def test_a_closed_context_is_refused(fake, own):
     ctx.close()
 
 
+def test_contexts_on_one_stream(fake):
+    a, b, c, d = (fake.context(s) for s in (None, None, 0x500, 0x600))
+    assert a.same_stream(b) and a.same_stream(a) and c.same_stream(fake.context(0x500))
+    assert not a.same_stream(c) and not c.same_stream(a) and not c.same_stream(d)
+    b.index = 1
+    assert not a.same_stream(b)
+
+
 def test_the_stream_word_of_no_context():
     from molten_b200 import build
     build.build()

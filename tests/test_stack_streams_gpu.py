@@ -67,3 +67,21 @@ def test_a_cache_with_fewer_pages_than_the_batch_is_refused(cuda_ctx):
     with pytest.raises(ValueError, match="fewer pages"):
         build(5)
     build(4)
+
+
+def test_a_batch_of_another_stream_is_refused(cuda_ctx):
+    """Its plan would run beside the steps; another context on the same stream is fine."""
+    layers, head, embed = make_layers(421, 1, (0,), 5, torch.bfloat16)
+    stream = torch.cuda.Stream()
+    own, same, plain = lfm.Context(0, stream), lfm.Context(0, stream), lfm.Context(0)
+    try:
+        build = lambda a, b: DecodeStack(a, layers, head, embed, 1, n_experts=E, kv=kv.PagedBatch(b, 1, 5, BS, 5))  # noqa: E731
+        for a, b in ((cuda_ctx, own), (own, cuda_ctx)):
+            with pytest.raises(ValueError, match="another stream"):
+                build(a, b)
+        build(cuda_ctx, plain)
+        build(own, same)
+    finally:
+        torch.cuda.synchronize()
+        for c in (own, same, plain):
+            c.close()
