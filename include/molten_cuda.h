@@ -382,6 +382,7 @@ int mc_rope_turns(float theta, float position_scale, int rot_dim, uint64_t* out)
  * parts of one fused projection row. q_out is q itself, with its stride, or
  * apart from q, k and v; all four lie outside the cache. Angles are exact modulo
  * a turn at any position.
+ * The pages of k_cache and v_cache share no byte unless v is NULL.
  * Every row of q_out is written, also those without a slot. Slots are
  * distinct; of two tokens with one slot either may stay, or parts of both. */
 int mc_qk_norm_rope(mc_ctx* ctx, const uint16_t* q, size_t q_stride, const uint16_t* k,

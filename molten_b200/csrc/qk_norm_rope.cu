@@ -288,7 +288,7 @@ bool overlap(const void* p, size_t bytes, const void* q, size_t more) {
   return p && q && a < b + more && b < a + bytes;
 }
 
-// Of `tokens` rows of `an` bytes at a and of `bn` bytes at b, one each `a_step` / `b_step` bytes,
+// Of `tokens` rows (or pages) of `an` bytes at a and of `bn` bytes at b, one each `a_step` / `b_step` bytes,
 // some share a byte. Rows of one step may interleave (parts of one fused row); of two steps,
 // their whole ranges count.
 bool rows_overlap(const void* a, size_t an, size_t a_step, const void* b, size_t bn, size_t b_step,
@@ -361,6 +361,11 @@ extern "C" int mc_qk_norm_rope(mc_ctx* ctx, const uint16_t* q, size_t q_stride, 
   const size_t size = kv_dtype == MC_DTYPE_BF16 ? 2 : 1;  // bytes of an element
   const size_t cache_bytes = size * (block_stride * ((size_t)num_blocks - 1) +
                                      (size_t)n_kv_heads * block_size * head_dim);
+  // K's and V's pages may alternate, but share no byte (V NULL: one may stand for both)
+  const size_t page_bytes = size * ((size_t)n_kv_heads * block_size * head_dim);
+  MC_REQUIRE(!v || !rows_overlap(k_cache, page_bytes, size * block_stride, v_cache, page_bytes,
+                                 size * block_stride, (size_t)num_blocks),
+             "%s: k_cache overlaps v_cache", name);
   const void* const rows[4] = {q, k, v, q_out};
   const size_t bytes[4] = {2 * qn, 2 * kn, 2 * kn, 2 * qn};
   const size_t steps[4] = {q_step, 2 * k_stride, 2 * v_stride, out_step};
