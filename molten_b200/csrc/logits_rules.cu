@@ -14,8 +14,9 @@
 // every rule on, instructions, some 40 a token and lane. A thread takes 8
 // tokens: one 16-byte load of bf16 logits, one of counts, one byte of each
 // bitmap, the next span's on their way while it works on one (48 rows of
-// 128000 from HBM, 38 MB with all rules: 13.6 us; without biases and penalties,
-// 25 MB, 8.3 us; two spans ahead 1 us more). A CTA takes a few spans of 2048
+// 128000, 38 MB with all rules, of which the 26 MB that are read come from
+// DRAM: 13.6 us; without biases and penalties, 25 MB, 8.0 us; two spans ahead
+// 1 us more). A CTA takes a few spans of 2048
 // tokens of one row, so that a large batch is one wave. Biases are a short
 // sorted list a row; each CTA looks through the part that can fall into its
 // tokens (256 probes narrow a long list) and the thread at the first of a run
@@ -28,7 +29,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kSpan = 8 * kThreads;  // tokens a CTA takes at once
 constexpr int kSpans = 4;            // most spans of a CTA
-constexpr int kSpansBiased = 5;      // with biases
+constexpr int kSpansBiased = 5;      // with biases, in one wave
 constexpr int kResident = 5;         // CTAs an SM holds at once
 
 struct RulesParams {
@@ -369,14 +370,17 @@ extern "C" int mc_logits_process(mc_ctx* ctx, const void* logits, size_t logits_
                    (batch == 1 || logits_stride % lane == out_stride % lane) &&
                    (!counts || ((uintptr_t)counts / 2 % lane == la && mc_aligned(counts, 2) &&
                                 (batch == 1 || (size_t)vocab % lane == logits_stride % lane)));
-  // CTAs a row: as many as one wave leaves it, in runs of at most 4 spans; 5 with biases, whose
-  // layout a second wave repeats (48 rows of 128000 with the token tail: 624 CTAs of 5 spans 16.3
-  // us, 768 of 4 16.9; without biases 15.2 and 14.7)
+  // CTAs a row: as many as one wave leaves it, in runs of at most 4 spans; 5 with biases where that
+  // makes one wave, since a second one would zero and fill its shared memory once more. With the
+  // token tail, runs of 5 and of 4: one wave by fives, two by fours: 50 rows of 128000 16.4 and 17.6
+  // us, 56 of 128000 16.0 and 18.3, 100 of 65536 16.7 and 18.5; two waves either way: 64 of 128000
+  // 21.1 and 19.8, 128 of 65536 22.3 and 21.4, 256 of 32000 23.5 and 21.3; without biases 48 of
+  // 128000 15.2 and 14.6, 128 of 128000 28.9 and 27.2 (by threes 30.2). 5 spans are the most whose
+  // shared memory (8 KB each) kResident CTAs hold.
   const int all = (vocab + (vec ? (int)lane - 1 : 0) + kSpan - 1) / kSpan;
   const int share = kResident * ctx->num_sms / batch;
-  const int most = bias_start ? kSpansBiased : kSpans;
-  int spans = share > 0 ? (all + share - 1) / share : most;
-  spans = spans < 1 ? 1 : spans > most ? most : spans;
+  const int spans_of_a_wave = share > 0 ? (all + share - 1) / share : all;
+  const int spans = spans_of_a_wave <= (bias_start ? kSpansBiased : kSpans) ? spans_of_a_wave : kSpans;
   P.spans = spans;
   const dim3 grid((unsigned)((all + spans - 1) / spans), (unsigned)batch);
   auto fn = dtype == MC_DTYPE_F32
