@@ -244,12 +244,13 @@ paged_attention_kernel(const PaParams P) {
   const int capacity = P.capacity;
   const int cta = blockIdx.x;
 
-  auto row_of = [&](int r) {
-    int len = P.kv_lens[r];
+  auto row_of = [&](int r, int* of = nullptr) {
+    int len = P.kv_lens[r], req = r;
     if (P.row_req) {
-      const int req = P.row_req[r];
-      if (req < 0 || req >= P.n_req) len = 0;
+      req = P.row_req[r];
+      if (req < 0 || req >= P.n_req) len = req = 0;
     }
+    if (of) *of = req;
     return ps_row(len, capacity, P.window);
   };
   int unit = P.small_unit;  // keys of a unit
@@ -321,12 +322,13 @@ paged_attention_kernel(const PaParams P) {
   bool more = true;
   const int32_t* table = nullptr;
   auto enter = [&]() {  // the piece `fill`
-    const PsRow keys = row_of(fill.row);
+    int req;  // read once: a table row that is there, whatever changes meanwhile
+    const PsRow keys = row_of(fill.row, &req);
     const int lo = keys.low + fill.unit * unit;
     fill_hi = (int)min((long long)keys.len, (long long)lo + (long long)fill.units * unit);
     fill_base = lo + warp * S::kStep;
     head_row = (uint32_t)(fill.item / P.subs) * P.block_size;
-    table = P.table + (size_t)(P.row_req ? max(P.row_req[fill.row], 0) : fill.row) * P.width;
+    table = P.table + (size_t)req * P.width;
   };
   // to the next step of this warp; its page numbers are on their way afterwards
   auto seek = [&]() {
