@@ -402,8 +402,12 @@ int mc_qk_norm_rope(mc_ctx* ctx, const uint16_t* q, size_t q_stride, const uint1
  * (or with row_req -1) gives zeros and lse -inf. Several rows of one request
  * (draft tokens, a short prompt) read their keys each for itself. Keys of
  * pages outside [0, num_blocks) are left out; nothing behind kv_lens is read.
- * A non-finite K or V element of a key that is read makes the results it
- * enters non-finite. out must not overlap q. workspace: zeroed once,
+ * A NaN in K or V of a key that is read, an infinite V or a score of +inf makes
+ * the results it enters NaN or infinite; a score of -inf weighs its key with
+ * zero.
+ * out must not overlap q. kv_lens and row_req must not change while the call
+ * runs: that gives wrong results, though no access out of range, and the
+ * workspace has to be zeroed again. workspace: zeroed once,
  * mc_paged_attention_workspace_bytes(head_dim) device bytes, 16-byte aligned,
  * owned by one chain of ordered calls (each call leaves its counters zero
  * again; captured graphs that may run at once need one each). */

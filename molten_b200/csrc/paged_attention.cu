@@ -22,10 +22,12 @@
 // Memory. Every warp has a ring of steps in shared memory that its own lanes
 // fill with 16-byte asynchronous copies, deep enough that an SM has 60 KB and
 // more on their way, and filled across the borders of pieces, so that the next
-// item's keys arrive while the last one is joined. (1-D bulk copies, one for
-// each run of keys that lie together in a page, took as long for pages of 16
-// keys and up, 14% longer for e4m3 rows of 64 bytes, and 1.7 times as long for
-// pages of one key: a copy costs an SM some 47 cycles whatever its size.)
+// item's keys arrive while the last one is joined. (An earlier form of this
+// kernel filled the ring by 1-D bulk copies, one for each run of keys that lie
+// together in a page. When the two were compared they took as long for pages
+// of 16 keys and up, bulk copies 14% longer for e4m3 rows of 64 bytes and 1.7
+// times as long for pages of one key: a copy cost an SM some 47 cycles
+// whatever its size.)
 //
 // Rounding of P. P is split into high and low parts (bf16 + bf16, or f16 + f16
 // for an e4m3 cache), so it enters the product with 16 bits or more and the
@@ -39,7 +41,8 @@
 // of the 16-row tile, and the low parts ride in rows 8-15 at no cost; where
 // more than 8 heads share a KV head a tile takes 16 and the low parts cost
 // products of their own (16 heads a KV head, 64 rows of 4000 to 8200 keys of
-// 128: 472 us by eights, 250 us by sixteens; e4m3 277 and 176 us).
+// 128: 464 us by eights, 245 us by sixteens, e4m3 273 and 172; of 64: 247 and
+// 129, e4m3 161 and 116).
 // With an e4m3 cache K and V become f16 exactly, and Q becomes f16 scaled by
 // a power of two a row (its largest value near 1), which loses nothing above
 // 2^-24 of that value.
@@ -172,10 +175,13 @@ __device__ __forceinline__ void e4m3x4_to_f16(uint32_t v, uint32_t& lo, uint32_t
 
 // Shape of the kernel for a head dimension and cache type: 8 warps an SM with
 // rings that hold 128 to 192 KB, except e4m3 rows of 64 bytes, whose time goes
-// into instructions more than into bytes and which take 12 warps (97 -> 85 us
-// for 64 rows of 6100 keys x 8 heads; bf16 rows at 12 warps and shallower rings
-// 51 -> 54 us for 131071 keys). Rows of 256 bytes take 16 keys a step, so that
-// 4 warps' rings fit twice (94 -> 87 us for 131071 keys).
+// into instructions more than into bytes and which take 12 warps (64 rows of
+// 4000 to 8200 keys: 100 us with 8, 86 with 12; 131071 keys 43.4 and 39.3).
+// bf16 rows of 64 at 12 warps and two steps a ring: 131071 keys 51.4 -> 50.4
+// us, 32 rows of 17 to 6000 keys 40.8 -> 39.0, 64 rows of 4000 to 8200 keys
+// 126.1 -> 127.1. Rows of 256 bytes take 16 keys a step, so that 4 warps' rings
+// fit twice (131071 keys: 99.6 us with 32 keys a step and one CTA an SM, 90.9
+// with 16 and two; 64 rows of 4000 to 8200 keys 257 and 239).
 //
 // A step's K, and its V, are 128-byte lines of 8 chunks (16 bytes; chunk ch of
 // key k is number k kChunks + ch). A line's chunks are permuted, number n at

@@ -211,7 +211,8 @@ def qk_norm_rope(ctx: Context, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
 
 
 def paged_attention_workspace(head_dim: int, device="cuda") -> torch.Tensor:
-    """A zeroed workspace of paged_attention, for one chain of ordered calls."""
+    """A workspace of paged_attention, for one chain of ordered calls, zeroed on
+    the current stream. Zero it again if lengths or rows changed while a call ran."""
     n = int(_lib.lib().mc_paged_attention_workspace_bytes(head_dim))
     ensure(n > 0, f"paged_attention: head_dim {head_dim} (64 and 128 are built)")
     return torch.zeros(n, dtype=torch.uint8, device=device)
