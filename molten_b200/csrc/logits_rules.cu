@@ -16,8 +16,8 @@
 // bitmap, the next span's on their way while it works on one (48 rows of
 // 128000, 38 MB with all rules, of which the 26 MB that are read come from
 // DRAM: 13.6 us; without biases and penalties, 25 MB, 8.0 us; two spans ahead
-// 1 us more). A CTA takes a few spans of 2048
-// tokens of one row, so that a large batch is one wave. Biases are a short
+// 1 us more). A CTA takes a few spans of 2048 tokens of one row, so that a
+// large batch is one wave. Biases are a short
 // sorted list a row; each CTA looks through the part that can fall into its
 // tokens (256 probes narrow a long list) and the thread at the first of a run
 // of equal ids adds the run up into shared memory, so no order of atomics

@@ -37,9 +37,8 @@
 // the largest one of the warp's keys, fewer below, and none below 2^-40 (with
 // a largest weight of 1 a key of weight 2^-25 counted nothing, and one that
 // outweighs a long flat tail but has V near zero left a result that was off by
-// its own size). Eight heads fill rows 0-7
-// of the 16-row tile, and the low parts ride in rows 8-15 at no cost; where
-// more than 8 heads share a KV head a tile takes 16 and the low parts cost
+// its own size). Eight heads fill rows 0-7 of the 16-row tile, and the low
+// parts ride in rows 8-15 at no cost; where more than 8 heads share a KV head a tile takes 16 and the low parts cost
 // products of their own (16 heads a KV head, 64 rows of 4000 to 8200 keys of
 // 128: 464 us by eights, 245 us by sixteens, e4m3 273 and 172; of 64: 247 and
 // 129, e4m3 161 and 116).

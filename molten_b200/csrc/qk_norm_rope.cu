@@ -16,15 +16,15 @@
 //
 // What bounds it: latency (the launch, the angles and first rows of a CTA, which
 // nothing overlaps) and instructions, 52% of issue slots for a prompt's rows;
-// each row is read once and written once. A thread holds 8 elements of one head row, the two groups of 4
-// that rotate into each other (so no pair crosses threads), for every token of
-// the CTA's batch: its gains, addresses and role stay in registers. A batch's
-// cosines, sines and cache rows are computed once into shared memory by all
-// threads together. One wave of CTAs shares the tokens evenly, in batches of
-// up to 16, with 4 tokens' loads in flight, each asked for as soon as the one
-// in its place is unpacked (4096 tokens of 32 + 2 x 8 heads of 64, 50 MB, of
-// which the 25 MB that are read come from DRAM at a quarter of its rate: 12.7
-// us; 4 loaded together after 4 are done, in batches of 8, 14.6; 3 CTAs an SM
+// each row is read once and written once. A thread holds 8 elements of one head
+// row, the two groups of 4 that rotate into each other (so no pair crosses
+// threads), for every token of the CTA's batch: its gains, addresses and role
+// stay in registers. A batch's cosines, sines and cache rows are computed once
+// into shared memory by all threads together. One wave of CTAs shares the
+// tokens evenly, in batches of up to 16, with 4 tokens' loads in flight, each
+// asked for as soon as the one in its place is unpacked (4096 tokens of 32 + 2
+// x 8 heads of 64, 50 MB, of which the 25 MB that are read come from DRAM at a
+// quarter of its rate: 12.7 us; 4 loaded together after 4 are done, in batches of 8, 14.6; 3 CTAs an SM
 // with 2 in flight each 13.0; a CTA a token, rotation partners by shuffle,
 // 25.6).
 #include <cuda_fp8.h>
